@@ -74,7 +74,7 @@ def reference_symbols() -> list[str]:
 
 def build_ref_cpu() -> Path | None:
     """The reference's CPU references, callable: pins h3_oracle.c."""
-    if not REF.is_dir():
+    if not (REF / "h3_gpu.h").exists():
         return None
     OUT.mkdir(exist_ok=True)
     target = OUT / "libh3refcpu.so"
@@ -107,7 +107,7 @@ def build_ref_cpu() -> Path | None:
 
 def build_ref_cuda() -> Path | None:
     """The reference's own CUDA backend as a separate library (GPU oracle)."""
-    if not REF.is_dir() or shutil.which("nvcc") is None:
+    if not (REF / "h3_gpu.h").exists() or shutil.which("nvcc") is None:
         return None
     OUT.mkdir(exist_ok=True)
     target = OUT / "libh3ref.so"
@@ -130,7 +130,7 @@ def build_ref_cuda() -> Path | None:
 
 def build_ref_tests(product_lib: Path) -> list[Path]:
     """The reference's own op test program, linked against the B200 library."""
-    if not REF.is_dir() or not product_lib.exists():
+    if not (REF / "h3_gpu.h").exists() or not product_lib.exists():
         return []
     OUT.mkdir(exist_ok=True)
     built = []
@@ -151,7 +151,7 @@ def build_ref_hosts(product_lib: Path) -> list[Path]:
     samplers), compiled unmodified from the reference tree, plus the small driver
     tests/dit_host_driver.c, linked once against the B200 library and once against the
     reference's CUDA backend: the same host code on both backends."""
-    if not REF.is_dir() or not product_lib.exists():
+    if not (REF / "h3_gpu.h").exists() or not product_lib.exists():
         return []
     OUT.mkdir(exist_ok=True)
     units = ["h3_dit.c", "h3_dit_schedule.c", "h3_host.c", "h3_weights.c", "h3_safetensors.c"]
@@ -189,7 +189,7 @@ def build_ref_vae_hosts(product_lib: Path) -> list[Path]:
     chunks and blending), compiled unmodified from the reference tree, plus the small driver
     tests/vae_host_driver.c, linked once against the B200 library and once against the
     reference's CUDA backend."""
-    if not REF.is_dir() or not product_lib.exists():
+    if not (REF / "h3_gpu.h").exists() or not product_lib.exists():
         return []
     OUT.mkdir(exist_ok=True)
     units = ["h3_video_vae.c", "h3_weights.c", "h3_safetensors.c"]
