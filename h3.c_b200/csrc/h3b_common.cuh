@@ -164,6 +164,41 @@ inline int h3b_need(h3_gpu *gpu, const h3_gpu_tensor *t, h3_gpu_dtype dtype, siz
 
 void *h3b_workspace(h3_gpu *gpu, size_t bytes);
 
+/* Scratch of one call of the adapter and conditioning operators: the context's workspace, or, while
+ * the stream is being captured, memory that belongs to the graph (an allocation node, freed by a node
+ * behind the call's kernels), so that no two graphs and no later growth of the workspace can touch
+ * it. Null on failure; release goes behind the last launch that uses the block. */
+struct h3b_scratch {
+    h3_gpu *gpu;
+    void *data = nullptr;
+    bool captured = false;
+    h3b_scratch(h3_gpu *context, size_t bytes) : gpu(context) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        captured = cudaStreamIsCapturing(gpu->stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+        if (!captured) { data = h3b_workspace(gpu, bytes); return; }
+        if (cudaMallocAsync(&data, bytes ? bytes : 1, gpu->stream) != cudaSuccess) { cudaGetLastError(); data = nullptr; }
+    }
+    ~h3b_scratch() { if (captured && data) cudaFreeAsync(data, gpu->stream); }
+    h3b_scratch(const h3b_scratch &) = delete;
+    h3b_scratch &operator=(const h3b_scratch &) = delete;
+};
+
+/* The context's device for the length of a call, whatever device the calling thread has current */
+struct h3b_on_device {
+    int before = -1;
+    explicit h3b_on_device(const h3_gpu *gpu) {
+        int now = -1;
+        if (gpu && cudaGetDevice(&now) == cudaSuccess && now != gpu->device && cudaSetDevice(gpu->device) == cudaSuccess)
+            before = now;
+    }
+    ~h3b_on_device() { if (before >= 0) cudaSetDevice(before); }
+};
+
+inline bool h3b_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
 template <class T>
 inline T *h3b_ptr(const h3_gpu_tensor *t, size_t offset = 0) {
     return reinterpret_cast<T *>(t->data) + offset;

@@ -438,6 +438,46 @@ int h3x_linear_swiglu_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tens
                            const h3_gpu_tensor *fc1_weight, uint32_t rows, uint32_t input_dim,
                            uint32_t hidden_dim);
 
+/* ---- low-rank adapters of many requests beside a shared projection -----------------------------
+ * No counterpart in the reference, whose h3_gpu_linear_bf16 this stands beside. For every row r with
+ * a = row_adapter[r]:
+ *   output[r] = bf16( input[r] . weight^T + bias + scale[a] * ((input[r] . down[a]^T) . up[a]^T) )
+ * and without the last term where a >= adapters (0xffffffff by convention: a row without an adapter).
+ * Sums are F32; scale[a] * (input[r] . down[a]^T) is rounded to BF16 before it is multiplied by up on
+ * the tensor cores. BF16: input [rows][input_dim], weight [output_dim][input_dim], bias [output_dim] or
+ * NULL, down [adapters][rank][input_dim], up [adapters][output_dim][rank], output [rows][output_dim].
+ * scale is F32 [adapters] or NULL (all 1); row_adapter is U32 [rows] or NULL (every row has adapter 0).
+ * Adapters of a smaller rank are padded with zeros to `rank`. Rows of one request need not be
+ * contiguous; a row never depends on another row's adapter, whatever that adapter's weights hold.
+ * rank 1..256, adapters 0..1024 (0: the plain projection, down / up / scale are not looked at).
+ * output must not overlap any input. Counted like a projection of its shape. */
+int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                         const h3_gpu_tensor *weight, const h3_gpu_tensor *bias,
+                         const h3_gpu_tensor *down, const h3_gpu_tensor *up,
+                         const h3_gpu_tensor *scale, const h3_gpu_tensor *row_adapter,
+                         uint32_t rows, uint32_t input_dim, uint32_t output_dim, uint32_t adapters,
+                         uint32_t rank);
+
+/* ---- cross attention: query rows to an encoder's states of another length ----------------------
+ * No counterpart in the reference, whose h3_gpu_sdpa_bf16 this stands beside. `segments` is U32
+ * [segment_count][4]: first query row, query rows, first key row, key rows of one request. Within a
+ * segment every query row of head h attends every key row of head h / (heads / kv_heads):
+ *   output = softmax(query . key^T * scale) . value,   zeros where a segment has no keys.
+ * query and output are [query_rows][heads][head_dim], key and value [key_rows][kv_heads][head_dim],
+ * BF16; sums and softmax statistics are F32, probabilities are rounded to BF16 before they are
+ * multiplied by value on the tensor cores. segments == NULL: one segment of all rows (segment_count
+ * must be 0). Segments may share key rows and may leave gaps anywhere (states padded to one length);
+ * their query rows must not overlap. Query rows in no segment are left as they were; rows of a
+ * segment past query_rows or key_rows are ignored; what padding rows hold (infinities and NaN
+ * included) never reaches an output. heads must divide by kv_heads; head_dim up to 512 (64 and 128 with
+ * 16-byte aligned tensors and scale > 0 run on the tensor cores). output may be the query tensor
+ * itself; it must not overlap key or value. */
+int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,
+                        const h3_gpu_tensor *key, const h3_gpu_tensor *value,
+                        const h3_gpu_tensor *segments, uint32_t segment_count, uint32_t query_rows,
+                        uint32_t key_rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                        float scale);
+
 /* Declares that an F32 tensor serves as a projection weight (on != 0) or no longer does (0).
  * h3_gpu_linear_f32 keeps the scaled FP16 rows of such a weight between calls instead of
  * converting it every time; tensors made by h3_gpu_tensor_load_f32 / h3_gpu_tensor_from_f32 are
