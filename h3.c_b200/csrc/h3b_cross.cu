@@ -1,13 +1,17 @@
 /* Cross attention: query rows of several requests to an encoder's states of other lengths.
  *
- * h3b_cross_simt takes any head size, alignment and scale: one CTA per (query row, head) walks the keys
- * of the row's segment with the online softmax recurrence in F32.
+ * h3b_cross_tc (head_dim 64 and 128) runs on the tensor cores, described at its definition;
+ * h3b_cross_merge joins its partial results where the keys of a segment are split. h3b_cross_simt takes
+ * any head size, alignment and scale: one CTA per (query row, head) walks the keys of the row's segment
+ * with the online softmax recurrence in F32.
  */
 #include "h3b_common.cuh"
+#include "h3b_sm100.cuh"
 
 #include <cuda_bf16.h>
 
 #include <cmath>
+#include <cstdlib>
 
 namespace {
 
@@ -107,6 +111,630 @@ h3b_cross_simt(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t
     }
 }
 
+
+/* ------------------------------------------------------------- tensor cores
+ * A query tile is 128 rows of tensor memory: 128 / pack query rows of `pack` neighbouring heads that
+ * share a key head (pack = the largest power of two in heads / kv_heads), so that shared key heads are
+ * read once per tile. A work unit is GROUPS neighbouring tiles of one segment and head set over a range of
+ * 128-key tiles; one persistent CTA per SM (GROUPS 2) walks units w, w + grid, ...
+ *
+ *   warp 0   TMA: the unit's query tiles into one of QBUF buffers per group, K and V tiles through one
+ *            ring in the order K0 V0 K1 V1 ..., shared by the groups.
+ *   warp 1   tcgen05.mma: per step and group O += P.V, then the group's next scores Q.K^T. The next
+ *            step may belong to the next unit, so the tensor pipe never drains between units: states
+ *            are short (one to four steps), and a CTA per tile spends half of its time filling and
+ *            draining. P (BF16) overwrites the scores it came from and is the A operand of P.V; the
+ *            in-order pipe keeps the next scores behind it.
+ *   warps 2+ softmax, 4 warps per group: a thread owns one row. Scores of a step complete imply that
+ *            the group's P.V before them is complete (issued earlier on one pipe), so a raise of the
+ *            reference maximum may rescale O at once. While one group computes exponentials, the
+ *            tensor pipe works for the other.
+ * Keys past the segment get -inf scores by selection; value rows past it that belong to somebody else
+ * are cleared in shared memory before P.V reads them (0 * NaN is NaN).
+ * Tensor memory: S of group g at 128 g, O behind the scores. All waits are bounded. */
+constexpr int CT = 128;                              /* rows of a query tile, keys of a key tile */
+constexpr int CT_BOX = CT * 64 * 2;                  /* a TMA box: 128 rows x 64 dims            */
+constexpr float CT_RAISE = 8.0f;                     /* raise the reference by more than 2^8 only */
+
+template <int D> constexpr int ct_tile() { return CT * D * 2; }
+template <int D, int GROUPS> constexpr int ct_qbuf() { return GROUPS == 2 ? 2 : 1; }
+template <int D, int GROUPS> constexpr int ct_ring() { return GROUPS == 2 ? (D == 128 ? 3 : 8) : (D == 128 ? 2 : 4); }
+template <int GROUPS> constexpr int ct_threads() { return 64 + 128 * GROUPS; }
+template <int D, int GROUPS> constexpr size_t ct_smem() {
+    return size_t(GROUPS * ct_qbuf<D, GROUPS>() + ct_ring<D, GROUPS>()) * ct_tile<D>() + 512;
+}
+static_assert(ct_smem<128, 2>() <= 232448, "cross attention needs at most 227 KiB of shared memory");
+static_assert(2 * (ct_smem<128, 1>() + 1024) <= 233472, "two one-group CTAs per SM");
+
+struct CrossArgs {
+    uint16_t *out;
+    const uint32_t *segments;
+    float *partial_o, *partial_ml;       /* splits > 1: [split][query row][head][D], [split][query row][head][2] */
+    int *status;
+    long long wait_cycles;
+    uint32_t segment_count, query_rows, key_rows, heads, kv_heads;
+    uint32_t pack, pack_log2, head_units;    /* head_units = heads / pack */
+    uint32_t splits;
+    float scale_log2;
+};
+
+/* One work unit; every role walks the same units with a cursor of its own */
+struct CrossUnit {
+    uint32_t q_row, rows[2];     /* first query row; live query rows of each group's tile */
+    uint32_t head0, kv_head;
+    uint32_t k_row, keys;        /* first key row of the range; keys of the segment from there on */
+    uint32_t steps, split;
+    bool dirty;                  /* the last tile reaches rows that are not the segment's */
+};
+
+template <int GROUPS>
+struct CrossCursor {
+    uint32_t unit, index, before, items;
+    Segment segment;
+    __device__ __forceinline__ void enter(const CrossArgs &a) {
+        segment = load_segment(a.segments, index, a.query_rows, a.key_rows);
+        const uint32_t per_item = GROUPS * CT >> a.pack_log2;
+        items = (segment.queries + per_item - 1) / per_item;
+    }
+    __device__ __forceinline__ explicit CrossCursor(const CrossArgs &a) : unit(blockIdx.x), index(0), before(0) { enter(a); }
+    __device__ __forceinline__ bool next(const CrossArgs &a, CrossUnit &u) {
+        const uint32_t head_unit = unit % a.head_units, rest = unit / a.head_units;
+        const uint32_t item = rest / a.splits;
+        while (item - before >= items) {
+            before += items;
+            if (++index >= a.segment_count) return false;
+            enter(a);
+        }
+        unit += gridDim.x;
+        const uint32_t tile_rows = CT >> a.pack_log2, first = (item - before) * GROUPS * tile_rows;
+        u.q_row = segment.q0 + first;
+        u.rows[0] = min(tile_rows, segment.queries - first);
+        u.rows[1] = GROUPS == 2 && segment.queries - first > tile_rows ? min(tile_rows, segment.queries - first - tile_rows) : 0;
+        u.head0 = head_unit * a.pack;
+        u.kv_head = u.head0 / (a.heads / a.kv_heads);
+        u.split = rest % a.splits;
+        const uint32_t tiles = (segment.keys + CT - 1) / CT;
+        const uint32_t t0 = uint32_t(uint64_t(u.split) * tiles / a.splits), t1 = uint32_t(uint64_t(u.split + 1) * tiles / a.splits);
+        u.k_row = segment.k0 + t0 * CT;
+        u.keys = segment.keys - t0 * CT;
+        u.steps = t1 - t0;
+        u.dirty = t1 * uint64_t(CT) > segment.keys && segment.k0 + segment.keys < a.key_rows;
+        return true;
+    }
+};
+
+__device__ __forceinline__ void ct_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void ct_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ float ct_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+/* 32 scores -> 32 probabilities (16 packed columns), their sum added in two packed accumulators */
+__device__ __forceinline__ void ct_exponentials(const uint32_t *s, uint64_t scale2, uint64_t neg_m2, uint32_t (&packed)[16],
+                                                uint64_t &sum_a, uint64_t &sum_b) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint64_t xa = fma_f32x2(pack_f32x2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), scale2, neg_m2);
+        const uint64_t xb = fma_f32x2(pack_f32x2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), scale2, neg_m2);
+        float x0, x1, x2, x3;
+        unpack_f32x2(xa, x0, x1);
+        unpack_f32x2(xb, x2, x3);
+        const float p0 = ct_exp2(x0), p1 = ct_exp2(x1), p2 = ct_exp2(x2), p3 = ct_exp2(x3);
+        sum_a = add_f32x2(sum_a, pack_f32x2(p0, p1));
+        sum_b = add_f32x2(sum_b, pack_f32x2(p2, p3));
+        packed[2 * i] = pack_bf16(p0, p1);
+        packed[2 * i + 1] = pack_bf16(p2, p3);
+    }
+}
+
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(ct_threads<GROUPS>(), GROUPS == 2 ? 1 : 2)
+h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CrossArgs args) {
+    constexpr int TILE = ct_tile<D>(), QBUF = ct_qbuf<D, GROUPS>(), RING = ct_ring<D, GROUPS>();
+    constexpr uint32_t COL_O = GROUPS * CT, TMEM_COLS = GROUPS * 256;
+    extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
+    const uint32_t base = smem_u32(ct_smem_raw);
+    const uint32_t q_smem = base;                                   /* [group][buffer] */
+    const uint32_t ring_smem = q_smem + GROUPS * QBUF * TILE;
+    const uint32_t bars = ring_smem + RING * TILE;
+    const uint32_t q_full = bars;                                   /* [group][buffer] = 4 */
+    const uint32_t q_free = q_full + 32;                            /* [group][buffer] = 4 */
+    const uint32_t kv_full = q_free + 32;                           /* [stage] = 8         */
+    const uint32_t kv_free = kv_full + 64;                          /* [stage] = 8         */
+    const uint32_t s_full = kv_free + 64;                           /* [group]             */
+    const uint32_t p_full = s_full + 16;                            /* [group]             */
+    const uint32_t o_done = p_full + 16;                            /* [group]             */
+    const uint32_t holder = o_done + 16;
+    volatile int *stop = reinterpret_cast<volatile int *>(ct_smem_raw + (holder + 8 - base));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long budget = args.wait_cycles;
+    if ((base & 1023u) != 0) {       /* swizzled tiles need 1024-byte alignment */
+        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_ATTN_TIMEOUT));
+        return;
+    }
+    if (threadIdx.x == 0) {
+        *stop = 0;
+        for (int i = 0; i < GROUPS * QBUF; i++) { mbar_init(q_full + 8 * i, 1); mbar_init(q_free + 8 * i, 4); }
+        for (int i = 0; i < RING; i++) { mbar_init(kv_full + 8 * i, 1); mbar_init(kv_free + 8 * i, 1); }
+        for (int g = 0; g < GROUPS; g++) {
+            mbar_init(s_full + 8 * g, 1);
+            mbar_init(p_full + 8 * g, 4);
+            mbar_init(o_done + 8 * g, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
+    if (warp == 1) tmem_alloc(holder, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem_base;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(holder));
+
+    CrossCursor<GROUPS> cursor(args);
+    CrossUnit u;
+    if (warp == 0) {
+        /* ---------------------------------------------------------------- TMA producer */
+        if (lane == 0) {
+            uint32_t q_count[2] = {0, 0}, tile = 0;
+            bool alive = true;
+            /* K (kind 0) or V tile at key row `row` into the ring */
+            auto load_tile = [&](const CUtensorMap *map, uint32_t row) {
+                const uint32_t stage = tile % RING, round = tile / RING;
+                if (round && !mbar_wait(kv_free + 8 * stage, (round - 1) & 1u, stop, budget)) return false;
+                const uint32_t bar = kv_full + 8 * stage, dst = ring_smem + stage * TILE;
+                mbar_expect_tx(bar, TILE);
+                ct_load(dst, map, bar, 0, int(u.kv_head), int(row));
+                if (D == 128) ct_load(dst + CT_BOX, map, bar, 64, int(u.kv_head), int(row));
+                tile++;
+                return true;
+            };
+            while (alive && cursor.next(args, u)) {
+                if (!u.steps) continue;
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) {
+                    if (!alive || !u.rows[g]) continue;
+                    const uint32_t buffer = q_count[g] % QBUF, round = q_count[g] / QBUF;
+                    alive = !round || mbar_wait(q_free + 8 * (g * QBUF + buffer), (round - 1) & 1u, stop, budget);
+                    if (!alive) break;
+                    const uint32_t bar = q_full + 8 * (g * QBUF + buffer), dst = q_smem + (g * QBUF + buffer) * TILE;
+                    const int row = int(u.q_row + g * (CT >> args.pack_log2));
+                    mbar_expect_tx(bar, TILE);
+                    ct_load(dst, &map_q, bar, 0, int(u.head0), row);
+                    if (D == 128) ct_load(dst + CT_BOX, &map_q, bar, 64, int(u.head0), row);
+                    q_count[g]++;
+                    if (g == 0) alive = load_tile(&map_k, u.k_row);
+                }
+                for (uint32_t j = 0; alive && j < u.steps; j++) {
+                    if (j) alive = load_tile(&map_k, u.k_row + j * CT);
+                    alive = alive && load_tile(&map_v, u.k_row + j * CT);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        /* ------------------------------------------------------------------ MMA issuer */
+        const uint32_t leader = lane == 0;
+        constexpr uint32_t idesc_qk = instruction_desc(CT, CT);
+        constexpr uint32_t idesc_pv = instruction_desc(CT, D) | (1u << 16);     /* V is N-major */
+        constexpr uint32_t HALF = CT_BOX >> 4, STAGE = TILE >> 4;
+        const uint32_t q_lo0 = desc_lo_kmajor(q_smem), k_lo0 = desc_lo_kmajor(ring_smem);
+        const uint32_t v_lo0 = desc_lo_nmajor(ring_smem, CT_BOX);
+        uint32_t q_count[2] = {0, 0}, p_count[2] = {0, 0}, tile = 0;
+        bool alive = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, budget));
+            return alive;
+        };
+        /* scores of group g against the K tile in ring position `k_tile`; q_count was advanced at the
+         * unit's first step */
+        auto issue_qk = [&](int g, uint32_t k_tile) {
+            const uint32_t d = tmem_base + g * CT;
+            const uint32_t q_lo = q_lo0 + (g * QBUF + (q_count[g] - 1) % QBUF) * STAGE;
+            const uint32_t k_lo = k_lo0 + (k_tile % RING) * STAGE;
+            umma_ss<false>(d, q_lo, k_lo, idesc_qk, leader);
+#pragma unroll
+            for (int kk = 1; kk < D / 16; kk++)
+                umma_ss<true>(d, q_lo + (kk >> 2) * HALF + 2 * (kk & 3), k_lo + (kk >> 2) * HALF + 2 * (kk & 3), idesc_qk, leader);
+            umma_commit_if(s_full + 8 * g, leader);
+        };
+        /* the first unit with keys */
+        bool have = false;
+        while (!have && cursor.next(args, u)) have = u.steps != 0;
+        if (have && wait(kv_full + 8 * (tile % RING), (tile / RING) & 1u)) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                if (!u.rows[g]) continue;
+                if (!wait(q_full + 8 * (g * QBUF), 0)) break;
+                q_count[g]++;
+                tc_fence_after();
+                issue_qk(g, tile);
+            }
+            umma_commit_if(kv_free + 8 * (tile % RING), leader);
+        }
+        uint32_t j = 0;
+        while (alive && have) {
+            /* step j of unit u: its V tile is ring position tile + 1, the next step's K tile + 2 */
+            const uint32_t v_tile = tile + 1, k_tile = tile + 2;
+            const bool last = j + 1 == u.steps;
+            CrossUnit n = u;
+            bool more = true;
+            if (last) {
+                more = false;
+                while (!more && cursor.next(args, n)) more = n.steps != 0;
+            }
+            bool k_seen = false, v_seen = false;
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                if (alive && u.rows[g]) {
+                    if (!v_seen && !wait(kv_full + 8 * (v_tile % RING), (v_tile / RING) & 1u)) break;
+                    v_seen = true;
+                    if (!wait(p_full + 8 * g, p_count[g] & 1u)) break;
+                    p_count[g]++;
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + COL_O + g * D, a = tmem_base + g * CT;
+                    const uint32_t v_lo = v_lo0 + (v_tile % RING) * STAGE;
+                    if (j == 0) umma_ts<false>(d, a, v_lo, idesc_pv, leader);
+                    else umma_ts<true>(d, a, v_lo, idesc_pv, leader);
+#pragma unroll
+                    for (uint32_t kk = 1; kk < 8; kk++) umma_ts<true>(d, a + kk * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader);
+                    if (last) umma_commit_if(o_done + 8 * g, leader);
+                }
+                if (alive && more && n.rows[g]) {
+                    if (!k_seen && !wait(kv_full + 8 * (k_tile % RING), (k_tile / RING) & 1u)) break;
+                    k_seen = true;
+                    if (last) {
+                        if (!wait(q_full + 8 * (g * QBUF + q_count[g] % QBUF), (q_count[g] / QBUF) & 1u)) break;
+                        q_count[g]++;
+                    }
+                    tc_fence_after();
+                    issue_qk(g, k_tile);
+                }
+            }
+            if (!alive) break;
+            umma_commit_if(kv_free + 8 * (v_tile % RING), leader);
+            if (more) umma_commit_if(kv_free + 8 * (k_tile % RING), leader);
+            tile += 2;
+            have = more;
+            u = n;
+            j = last ? 0 : j + 1;
+        }
+    } else {
+        /* --------------------------------------------------------------------- softmax */
+        const int g = (warp - 2) >> 2;
+        const uint32_t quarter = warp & 3, local_row = quarter * 32 + lane, lane_base = (quarter * 32) << 16;
+        const uint32_t tmem_s = tmem_base + g * CT + lane_base, tmem_o = tmem_base + COL_O + g * D + lane_base;
+        const float scale_log2 = args.scale_log2;
+        const uint64_t scale2 = pack_f32x2(scale_log2, scale_log2);
+        uint32_t q_count = 0, s_count = 0, o_count = 0, tile = 0;
+        bool alive = true;
+        while (alive && cursor.next(args, u)) {
+            const uint32_t rows = g == 0 ? u.rows[0] : u.rows[1];
+            /* this thread's output row */
+            const uint32_t live = (local_row >> args.pack_log2) < rows;
+            const size_t row = size_t(u.q_row + g * (CT >> args.pack_log2) + (local_row >> args.pack_log2));
+            const uint32_t head = u.head0 + (local_row & (args.pack - 1));
+            if (!rows) { tile += 2 * u.steps; continue; }
+            if (!u.steps) {
+                /* no keys: zeros, or a part that weighs nothing */
+                if (live && args.splits == 1) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(args.out + (row * args.heads + head) * D);
+#pragma unroll
+                    for (int i = 0; i < D / 8; i++) dst[i] = make_uint4(0, 0, 0, 0);
+                } else if (live) {
+                    *reinterpret_cast<float2 *>(args.partial_ml + ((size_t(u.split) * args.query_rows + row) * args.heads + head) * 2) =
+                        make_float2(-INFINITY, 0.0f);
+                }
+                continue;
+            }
+            float reference = -INFINITY, sum = 0.0f;
+            for (uint32_t j = 0; j < u.steps; j++) {
+                alive = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, s_count & 1u, stop, budget));
+                if (!alive) break;
+                s_count++;
+                tc_fence_after();
+                const uint32_t valid = u.keys - j * CT;
+                /* GROUPS 2 holds the 128 scores in registers; with two CTAs per SM there is room for 32,
+                 * and they are read from tensor memory twice */
+                uint32_t s[GROUPS == 2 ? CT : 32];
+                float m_step = -INFINITY;
+                auto clip = [&](uint32_t *v, int first, int count) {
+                    if (valid < CT) {
+#pragma unroll
+                        for (int i = 0; i < count; i++)
+                            if (uint32_t(first + i) >= valid) v[i] = 0xff800000u;
+                    }
+                };
+                auto most_of = [&](const uint32_t *v, int count) {
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < count; i += 4) {
+                        m0 = max3_f32(m0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        m1 = max3_f32(m1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                    }
+                    return fmaxf(m0, m1);
+                };
+                if constexpr (GROUPS == 2) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) tmem_ld32(tmem_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                    tmem_ld_wait();
+                    clip(s, 0, CT);
+                    m_step = most_of(s, CT);
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld32(tmem_s + 32 * c, s);
+                        tmem_ld_wait();
+                        clip(s, 32 * c, 32);
+                        m_step = fmaxf(m_step, most_of(s, 32));
+                    }
+                }
+                m_step *= scale_log2;
+                const bool raise = m_step - reference > CT_RAISE;      /* true at the first finite score */
+                if (j > 0 && __any_sync(0xffffffffu, raise)) {
+                    const float alpha = raise ? ct_exp2(reference - m_step) : 1.0f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t o[32];
+                        tmem_ld32(tmem_o + c * 32, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st32(tmem_o + c * 32, o);
+                    }
+                    tmem_st_wait_all();
+                }
+                if (raise) {
+                    sum *= ct_exp2(reference - m_step);      /* 0 from -inf */
+                    reference = m_step;
+                }
+                /* a row whose scores are all -inf so far: probabilities 0, not exp2(-inf + inf) */
+                const float neg_m = reference == -INFINITY ? 0.0f : -reference;
+                const uint64_t neg_m2 = pack_f32x2(neg_m, neg_m);
+                uint64_t sum_a = 0, sum_b = 0;
+                if constexpr (GROUPS == 2) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t packed[16];
+                        ct_exponentials(s + 32 * c, scale2, neg_m2, packed, sum_a, sum_b);
+                        ct_st16(tmem_s + c * 16, packed);
+                    }
+                } else {
+                    /* P chunk c lands on columns 16 c .. 16 c + 15, in front of the scores still to be read */
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t packed[16];
+                        tmem_ld32(tmem_s + 32 * c, s);
+                        tmem_ld_wait();
+                        clip(s, 32 * c, 32);
+                        ct_exponentials(s, scale2, neg_m2, packed, sum_a, sum_b);
+                        ct_st16(tmem_s + c * 16, packed);
+                    }
+                }
+                if (g == 0 && u.dirty && j + 1 == u.steps) {
+                    /* value rows that are not the segment's: cleared before anybody's P.V, which is issued
+                     * behind this group's arrival */
+                    const uint32_t v_tile = tile + 2 * j + 1, stage = v_tile % RING;
+                    alive = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (v_tile / RING) & 1u, stop, budget));
+                    if (!alive) break;
+                    if (local_row >= valid) {
+                        const uint32_t at = ring_smem + stage * TILE + local_row * 128;
+#pragma unroll
+                        for (int i = 0; i < D / 8; i++)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                                         ::"r"(at + (i >> 3) * CT_BOX + (i & 7) * 16), "r"(0) : "memory");
+                    }
+                    fence_async_smem();
+                }
+                tmem_st_wait_all();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * g);
+                float s0, s1, s2, s3;
+                unpack_f32x2(sum_a, s0, s1);
+                unpack_f32x2(sum_b, s2, s3);
+                sum += (s0 + s1) + (s2 + s3);
+            }
+            if (!alive) break;
+            tile += 2 * u.steps;
+            alive = __all_sync(0xffffffffu, mbar_wait(o_done + 8 * g, o_count & 1u, stop, budget));
+            if (!alive) break;
+            o_count++;
+            tc_fence_after();
+            const uint32_t q_slot = g * QBUF + q_count % QBUF;
+            q_count++;
+            if (args.splits > 1) {
+                const size_t at = (size_t(u.split) * args.query_rows + row) * args.heads + head;
+                if (live) *reinterpret_cast<float2 *>(args.partial_ml + at * 2) = make_float2(reference, sum);
+#pragma unroll 1
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_o + c * 32, o);
+                    tmem_ld_wait();
+                    if (live) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            reinterpret_cast<uint4 *>(args.partial_o + at * D + c * 32)[i] =
+                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+            } else {
+                /* all scores -inf: zeros; a NaN sum stays NaN */
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                /* the tile's queries are not needed any more: their buffer turns rows held by threads into
+                 * whole-row stores (16-byte pieces, XOR-swizzled by row) */
+                constexpr uint32_t ROW_BYTES = D * 2, CHUNKS = D / 8, ROWS_PER_STORE = 32 / CHUNKS;
+                const uint32_t stage = q_smem + q_slot * TILE + quarter * 32 * ROW_BYTES;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_o + c * 32, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t v = 0; v < 4; v++) {
+                        const uint32_t at = stage + lane * ROW_BYTES + (((c * 4 + v) ^ (lane & (CHUNKS - 1))) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv)),
+                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv)),
+                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv)),
+                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv))
+                                     : "memory");
+                    }
+                }
+                __syncwarp();
+                const uint32_t chunk = lane & (CHUNKS - 1);
+#pragma unroll
+                for (uint32_t i = 0; i < CHUNKS; i++) {
+                    const uint32_t r = ROWS_PER_STORE * i + lane / CHUNKS, t = quarter * 32 + r;
+                    uint4 val;
+                    const uint32_t at = stage + r * ROW_BYTES + ((chunk ^ (r & (CHUNKS - 1))) << 4);
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(val.x), "=r"(val.y), "=r"(val.z), "=r"(val.w) : "r"(at) : "memory");
+                    if ((t >> args.pack_log2) < rows) {
+                        const size_t out_row = size_t(u.q_row + g * (CT >> args.pack_log2) + (t >> args.pack_log2));
+                        *reinterpret_cast<uint4 *>(args.out + (out_row * args.heads + u.head0 + (t & (args.pack - 1))) * D + chunk * 8) = val;
+                    }
+                }
+                fence_async_smem();
+            }
+            /* O has been read and the query buffer is done with: the next unit's P.V waits for this group's
+             * next P anyway, the next queries for this */
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_free + 8 * q_slot);
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*stop) {
+        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_ATTN_TIMEOUT));
+        /* give copies that may still be in flight time to land before the CTA retires */
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem_base, TMEM_COLS);
+    }
+}
+
+/* out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits in order, one warp per (row, head);
+ * rows of no segment are left alone. */
+template <int D>
+__global__ void __launch_bounds__(256)
+h3b_cross_merge(const CrossArgs args) {
+    const size_t unit = (size_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (unit >= size_t(args.query_rows) * args.heads) return;
+    const uint32_t lane = threadIdx.x & 31, row = uint32_t(unit / args.heads);
+    bool found = !args.segments;
+    for (uint32_t i = lane; !found && i < args.segment_count; i += 32) {
+        const Segment s = load_segment(args.segments, i, args.query_rows, args.key_rows);
+        found = row - s.q0 < s.queries;
+    }
+    if (!__any_sync(0xffffffffu, found)) return;
+    const size_t stride = size_t(args.query_rows) * args.heads;
+    float m = -INFINITY;
+    for (uint32_t s = 0; s < args.splits; s++) {
+        const float part = args.partial_ml[(s * stride + unit) * 2];
+        if (part > m || part != part) m = part;
+    }
+    float sum = 0.0f, o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) o[i] = 0.0f;
+    for (uint32_t s = 0; s < args.splits; s++) {
+        const float2 ml = *reinterpret_cast<const float2 *>(args.partial_ml + (s * stride + unit) * 2);
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;       /* nothing attended: its O was not written */
+        const float weight = ct_exp2(ml.x - m);
+        sum = fmaf(ml.y, weight, sum);
+        const float *src = args.partial_o + (s * stride + unit) * D;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) o[i] = fmaf(src[lane + 32 * i], weight, o[i]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) args.out[unit * D + lane + 32 * i] = to_bf16(o[i] * inv);
+}
+
+/* [rows][heads][D] BF16 as a 3-D tensor (dim, head, row); box = 64 dims x box_heads x box_rows */
+bool ct_map(CUtensorMap *map, const uint16_t *data, uint32_t rows, uint32_t heads, uint32_t dim, uint32_t box_heads,
+            uint32_t box_rows) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    cuuint64_t dims[3] = {dim, heads, rows};
+    cuuint64_t strides[2] = {cuuint64_t(dim) * 2, cuuint64_t(heads) * dim * 2};
+    cuuint32_t box[3] = {64, box_heads, box_rows};
+    cuuint32_t elem[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(data), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+/* cudaFuncSetAttribute belongs to a device; one answer per device and kernel */
+template <int D, int GROUPS>
+bool ct_configure(int device) {
+    static std::mutex mutex;
+    static bool done[64];
+    std::lock_guard<std::mutex> guard(mutex);
+    if (!done[device & 63]) {
+        if (cudaFuncSetAttribute(h3b_cross_tc<D, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(ct_smem<D, GROUPS>())) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        done[device & 63] = true;
+    }
+    return true;
+}
+
+template <int D, int GROUPS>
+int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k, const uint16_t *v) {
+    if (!ct_configure<D, GROUPS>(gpu->device)) return h3b_fail(gpu, "cannot reserve shared memory for the cross attention kernel");
+    CUtensorMap map_q, map_k, map_v;
+    if (!ct_map(&map_q, q, args.query_rows, args.heads, D, args.pack, CT >> args.pack_log2) ||
+        !ct_map(&map_k, k, args.key_rows, args.kv_heads, D, 1, CT) || !ct_map(&map_v, v, args.key_rows, args.kv_heads, D, 1, CT))
+        return h3b_fail(gpu, "cannot encode the cross attention tensor maps");
+    /* most units there can be: every segment may end in a part of a tile */
+    const uint64_t per_item = uint64_t(GROUPS) * CT >> args.pack_log2;
+    const uint64_t units = (args.query_rows / per_item + args.segment_count) * args.head_units * args.splits;
+    if (units > 0xffffffffull - gpu->sm_count * 2) return h3b_fail(gpu, "cross attention has too many tiles");
+    const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2);
+    const unsigned grid = unsigned(units < resident ? units : resident);
+    h3b_scratch scratch(gpu, args.splits > 1 ? size_t(args.splits) * args.query_rows * args.heads * (D + 2) * sizeof(float) : 0);
+    if (args.splits > 1) {
+        if (!scratch.data) return h3b_fail(gpu, "cross_sdpa_bf16: cannot allocate the partial results");
+        args.partial_o = static_cast<float *>(scratch.data);
+        args.partial_ml = args.partial_o + size_t(args.splits) * args.query_rows * args.heads * D;
+    }
+    h3b_cross_tc<D, GROUPS><<<grid, ct_threads<GROUPS>(), ct_smem<D, GROUPS>(), gpu->stream>>>(map_q, map_k, map_v, args);
+    if (args.splits > 1) {
+        const size_t warps = size_t(args.query_rows) * args.heads;
+        h3b_cross_merge<D><<<unsigned((warps + 7) / 8), 256, 0, gpu->stream>>>(args);
+    }
+    return h3b_launched(gpu, "cross_sdpa_bf16", H3B_SDPA);
+}
+
+bool env_on(const char *name) {
+    const char *v = getenv(name);
+    return v && *v && strcmp(v, "0") != 0;
+}
+
 }  // namespace
 
 extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,
@@ -119,6 +747,7 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
     if (heads % kv_heads) return h3b_fail(gpu, "cross attention heads must divide by the key heads");
     if (head_dim > uint32_t(kSimtThreads * kSimtMaxDimsPerThread))
         return h3b_fail(gpu, "cross attention head dimension is too large");
+    if (query_rows > 0x7ffffe00u || key_rows > 0x7ffffe00u) return h3b_fail(gpu, "cross attention has too many rows");
     if (heads > 65535) return h3b_fail(gpu, "cross attention has too many heads");
     if (!segments && segment_count) return h3b_fail(gpu, "cross attention segments tensor has the wrong dtype");
     const size_t q_count = size_t(query_rows) * heads * head_dim, k_count = size_t(key_rows) * kv_heads * head_dim;
@@ -141,6 +770,29 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
     const uint16_t *q = h3b_ptr<uint16_t>(query), *k = h3b_ptr<uint16_t>(key), *v = h3b_ptr<uint16_t>(value);
     uint16_t *out = h3b_ptr<uint16_t>(output);
 
+    const bool aligned = h3b_aligned16(q) && h3b_aligned16(k) && h3b_aligned16(v) && h3b_aligned16(out);
+    if ((head_dim == 64 || head_dim == 128) && aligned && key_rows && scale > 0.0f && !env_on("H3B_SDPA_SIMT")) {
+        CrossArgs args = {};
+        args.out = out;
+        args.segments = table;
+        args.status = gpu->status_device;
+        args.wait_cycles = gpu->wait_cycles;
+        args.segment_count = segment_count;
+        args.query_rows = query_rows;
+        args.key_rows = key_rows;
+        args.heads = heads;
+        args.kv_heads = kv_heads;
+        const uint32_t group = heads / kv_heads;
+        while (args.pack_log2 < 7 && group % (2u << args.pack_log2) == 0) args.pack_log2++;
+        args.pack = 1u << args.pack_log2;
+        args.head_units = heads / args.pack;
+        args.scale_log2 = scale * 1.4426950408889634f;
+        const bool few = query_rows <= uint64_t(segment_count) * (CT >> args.pack_log2);
+        args.splits = 1;
+        if (const char *force = getenv("H3B_CROSS_SPLITS")) args.splits = uint32_t(atoi(force));
+        if (few) return head_dim == 128 ? ct_launch<128, 1>(gpu, args, q, k, v) : ct_launch<64, 1>(gpu, args, q, k, v);
+        return head_dim == 128 ? ct_launch<128, 2>(gpu, args, q, k, v) : ct_launch<64, 2>(gpu, args, q, k, v);
+    }
     const size_t smem = (size_t(head_dim) + kSimtThreads) * sizeof(float);
     h3b_cross_simt<<<dim3(query_rows, heads), kSimtThreads, smem, gpu->stream>>>(
         q, k, v, out, table, segment_count, query_rows, key_rows, heads, kv_heads, head_dim, scale);
