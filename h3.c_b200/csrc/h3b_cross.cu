@@ -125,7 +125,9 @@ h3b_cross_simt(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t
  *            are short (one to four steps), and a CTA per tile spends half of its time filling and
  *            draining. P (BF16) overwrites the scores it came from and is the A operand of P.V; the
  *            in-order pipe keeps the next scores behind it.
- *   warps 2+ softmax, 4 warps per group: a thread owns one row. Scores of a step complete imply that
+ *   warps 2+ softmax, 8 warps per group: two threads own a row, each 64 of a step's 128 keys and half of
+ *            the output; they exchange their maxima through shared memory and a named barrier of their
+ *            two warps, which also carries the vote to go on. Scores of a step complete imply that
  *            the group's P.V before them is complete (issued earlier on one pipe), so a raise of the
  *            reference maximum may rescale O at once. While one group computes exponentials, the
  *            tensor pipe works for the other.
@@ -139,9 +141,11 @@ constexpr float CT_RAISE = 8.0f;                     /* raise the reference by m
 template <int D> constexpr int ct_tile() { return CT * D * 2; }
 template <int D, int GROUPS> constexpr int ct_qbuf() { return GROUPS == 2 ? 2 : 1; }
 template <int D, int GROUPS> constexpr int ct_ring() { return GROUPS == 2 ? (D == 128 ? 3 : 8) : (D == 128 ? 2 : 4); }
-template <int GROUPS> constexpr int ct_threads() { return 64 + 128 * GROUPS; }
+template <int GROUPS> constexpr int ct_threads() { return 64 + 256 * GROUPS; }
+constexpr int CT_BARS = 512;
+template <int GROUPS> constexpr int ct_xchg() { return GROUPS * 2 * CT * 4; }    /* [group][half][row] */
 template <int D, int GROUPS> constexpr size_t ct_smem() {
-    return size_t(GROUPS * ct_qbuf<D, GROUPS>() + ct_ring<D, GROUPS>()) * ct_tile<D>() + 512;
+    return size_t(GROUPS * ct_qbuf<D, GROUPS>() + ct_ring<D, GROUPS>()) * ct_tile<D>() + CT_BARS + ct_xchg<GROUPS>();
 }
 static_assert(ct_smem<128, 2>() <= 232448, "cross attention needs at most 227 KiB of shared memory");
 static_assert(2 * (ct_smem<128, 1>() + 1024) <= 233472, "two one-group CTAs per SM");
@@ -154,7 +158,10 @@ struct CrossArgs {
     long long wait_cycles;
     uint32_t segment_count, query_rows, key_rows, heads, kv_heads;
     uint32_t pack, pack_log2, head_units;    /* head_units = heads / pack */
+    uint32_t units_per_kv;                   /* head units that share a key head */
     uint32_t splits;
+    uint32_t step_h, step_s, step_i;         /* the grid as (head unit, split, item) digits */
+    uint32_t block_stores;                   /* whole tiles leave through map_out */
     float scale_log2;
 };
 
@@ -169,36 +176,49 @@ struct CrossUnit {
 
 template <int GROUPS>
 struct CrossCursor {
-    uint32_t unit, index, before, items;
+    uint32_t h, s, item;            /* the next unit: head unit (fastest), split, item (pair of tiles) */
+    uint32_t index, before, items;  /* the segment that item is looked for in, items in front of it, its items */
     Segment segment;
     __device__ __forceinline__ void enter(const CrossArgs &a) {
         segment = load_segment(a.segments, index, a.query_rows, a.key_rows);
         const uint32_t per_item = GROUPS * CT >> a.pack_log2;
-        items = (segment.queries + per_item - 1) / per_item;
+        items = (segment.queries + per_item - 1) >> ((GROUPS == 2 ? 8 : 7) - a.pack_log2);
     }
-    __device__ __forceinline__ explicit CrossCursor(const CrossArgs &a) : unit(blockIdx.x), index(0), before(0) { enter(a); }
+    __device__ __forceinline__ explicit CrossCursor(const CrossArgs &a) : index(0), before(0) {
+        h = blockIdx.x % a.head_units;
+        const uint32_t rest = blockIdx.x / a.head_units;
+        s = rest % a.splits;
+        item = rest / a.splits;
+        enter(a);
+    }
     __device__ __forceinline__ bool next(const CrossArgs &a, CrossUnit &u) {
-        const uint32_t head_unit = unit % a.head_units, rest = unit / a.head_units;
-        const uint32_t item = rest / a.splits;
         while (item - before >= items) {
             before += items;
             if (++index >= a.segment_count) return false;
             enter(a);
         }
-        unit += gridDim.x;
-        const uint32_t tile_rows = CT >> a.pack_log2, first = (item - before) * GROUPS * tile_rows;
+        const uint32_t tile_rows = CT >> a.pack_log2, first = (item - before) * GROUPS * tile_rows, left = segment.queries - first;
         u.q_row = segment.q0 + first;
-        u.rows[0] = min(tile_rows, segment.queries - first);
-        u.rows[1] = GROUPS == 2 && segment.queries - first > tile_rows ? min(tile_rows, segment.queries - first - tile_rows) : 0;
-        u.head0 = head_unit * a.pack;
-        u.kv_head = u.head0 / (a.heads / a.kv_heads);
-        u.split = rest % a.splits;
+        u.rows[0] = min(tile_rows, left);
+        u.rows[1] = GROUPS == 2 && left > tile_rows ? min(tile_rows, left - tile_rows) : 0;
+        u.head0 = h << a.pack_log2;
+        u.kv_head = a.units_per_kv == 1 ? h : h / a.units_per_kv;
+        u.split = s;
         const uint32_t tiles = (segment.keys + CT - 1) / CT;
-        const uint32_t t0 = uint32_t(uint64_t(u.split) * tiles / a.splits), t1 = uint32_t(uint64_t(u.split + 1) * tiles / a.splits);
+        uint32_t t0 = 0, t1 = tiles;
+        if (a.splits > 1) {
+            t0 = uint32_t(uint64_t(s) * tiles / a.splits);
+            t1 = uint32_t(uint64_t(s + 1) * tiles / a.splits);
+        }
         u.k_row = segment.k0 + t0 * CT;
         u.keys = segment.keys - t0 * CT;
         u.steps = t1 - t0;
-        u.dirty = t1 * uint64_t(CT) > segment.keys && segment.k0 + segment.keys < a.key_rows;
+        u.dirty = t1 == tiles && (segment.keys & (CT - 1)) && segment.k0 + segment.keys < a.key_rows;
+        h += a.step_h;
+        s += a.step_s;
+        item += a.step_i;
+        if (h >= a.head_units) { h -= a.head_units; s++; }
+        if (s >= a.splits) { s -= a.splits; item++; }
         return true;
     }
 };
@@ -214,6 +234,13 @@ __device__ __forceinline__ void ct_st16(uint32_t taddr, const uint32_t (&r)[16])
         "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void ct_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ float ct_exp2(float x) {
     float y;
@@ -243,7 +270,8 @@ __device__ __forceinline__ void ct_exponentials(const uint32_t *s, uint64_t scal
 template <int D, int GROUPS>
 __global__ void __launch_bounds__(ct_threads<GROUPS>(), GROUPS == 2 ? 1 : 2)
 h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CrossArgs args) {
+             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+             const __grid_constant__ CrossArgs args) {
     constexpr int TILE = ct_tile<D>(), QBUF = ct_qbuf<D, GROUPS>(), RING = ct_ring<D, GROUPS>();
     constexpr uint32_t COL_O = GROUPS * CT, TMEM_COLS = GROUPS * 256;
     extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
@@ -260,6 +288,7 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     const uint32_t o_done = p_full + 16;                            /* [group]             */
     const uint32_t holder = o_done + 16;
     volatile int *stop = reinterpret_cast<volatile int *>(ct_smem_raw + (holder + 8 - base));
+    volatile float *xchg = reinterpret_cast<volatile float *>(ct_smem_raw + (bars - base) + CT_BARS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long budget = args.wait_cycles;
     if ((base & 1023u) != 0) {       /* swizzled tiles need 1024-byte alignment */
@@ -268,17 +297,18 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     }
     if (threadIdx.x == 0) {
         *stop = 0;
-        for (int i = 0; i < GROUPS * QBUF; i++) { mbar_init(q_full + 8 * i, 1); mbar_init(q_free + 8 * i, 4); }
+        for (int i = 0; i < GROUPS * QBUF; i++) { mbar_init(q_full + 8 * i, 1); mbar_init(q_free + 8 * i, 8); }
         for (int i = 0; i < RING; i++) { mbar_init(kv_full + 8 * i, 1); mbar_init(kv_free + 8 * i, 1); }
         for (int g = 0; g < GROUPS; g++) {
             mbar_init(s_full + 8 * g, 1);
-            mbar_init(p_full + 8 * g, 4);
+            mbar_init(p_full + 8 * g, 8);
             mbar_init(o_done + 8 * g, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_out) : "memory");
     }
     if (warp == 1) tmem_alloc(holder, TMEM_COLS);
     tc_fence_before();
@@ -292,26 +322,26 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (warp == 0) {
         /* ---------------------------------------------------------------- TMA producer */
         if (lane == 0) {
-            uint32_t q_count[2] = {0, 0}, tile = 0;
+            uint32_t q_count[2] = {0, 0}, stage = 0, round = 0;
             bool alive = true;
-            /* K (kind 0) or V tile at key row `row` into the ring */
+            /* the K or V tile at key row `row` into the next ring stage */
             auto load_tile = [&](const CUtensorMap *map, uint32_t row) {
-                const uint32_t stage = tile % RING, round = tile / RING;
                 if (round && !mbar_wait(kv_free + 8 * stage, (round - 1) & 1u, stop, budget)) return false;
                 const uint32_t bar = kv_full + 8 * stage, dst = ring_smem + stage * TILE;
                 mbar_expect_tx(bar, TILE);
                 ct_load(dst, map, bar, 0, int(u.kv_head), int(row));
                 if (D == 128) ct_load(dst + CT_BOX, map, bar, 64, int(u.kv_head), int(row));
-                tile++;
+                if (++stage == RING) { stage = 0; round++; }
                 return true;
             };
             while (alive && cursor.next(args, u)) {
                 if (!u.steps) continue;
+                alive = load_tile(&map_k, u.k_row);      /* in front of the queries: the MMA warp waits for it first */
 #pragma unroll
                 for (int g = 0; g < GROUPS; g++) {
                     if (!alive || !u.rows[g]) continue;
-                    const uint32_t buffer = q_count[g] % QBUF, round = q_count[g] / QBUF;
-                    alive = !round || mbar_wait(q_free + 8 * (g * QBUF + buffer), (round - 1) & 1u, stop, budget);
+                    const uint32_t buffer = q_count[g] % QBUF, q_round = q_count[g] / QBUF;
+                    alive = !q_round || mbar_wait(q_free + 8 * (g * QBUF + buffer), (q_round - 1) & 1u, stop, budget);
                     if (!alive) break;
                     const uint32_t bar = q_full + 8 * (g * QBUF + buffer), dst = q_smem + (g * QBUF + buffer) * TILE;
                     const int row = int(u.q_row + g * (CT >> args.pack_log2));
@@ -319,7 +349,6 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     ct_load(dst, &map_q, bar, 0, int(u.head0), row);
                     if (D == 128) ct_load(dst + CT_BOX, &map_q, bar, 64, int(u.head0), row);
                     q_count[g]++;
-                    if (g == 0) alive = load_tile(&map_k, u.k_row);
                 }
                 for (uint32_t j = 0; alive && j < u.steps; j++) {
                     if (j) alive = load_tile(&map_k, u.k_row + j * CT);
@@ -335,169 +364,186 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         constexpr uint32_t HALF = CT_BOX >> 4, STAGE = TILE >> 4;
         const uint32_t q_lo0 = desc_lo_kmajor(q_smem), k_lo0 = desc_lo_kmajor(ring_smem);
         const uint32_t v_lo0 = desc_lo_nmajor(ring_smem, CT_BOX);
-        uint32_t q_count[2] = {0, 0}, p_count[2] = {0, 0}, tile = 0;
+        uint32_t q_count[2] = {0, 0}, p_phase[2] = {0, 0};
         bool alive = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            alive = alive && __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, budget));
+            alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, budget));
             return alive;
         };
-        /* scores of group g against the K tile in ring position `k_tile`; q_count was advanced at the
-         * unit's first step */
-        auto issue_qk = [&](int g, uint32_t k_tile) {
+        /* scores of group g against the K tile in ring stage `ks`; q_count was advanced at the unit's first step */
+        auto issue_qk = [&](int g, uint32_t ks) {
             const uint32_t d = tmem_base + g * CT;
-            const uint32_t q_lo = q_lo0 + (g * QBUF + (q_count[g] - 1) % QBUF) * STAGE;
-            const uint32_t k_lo = k_lo0 + (k_tile % RING) * STAGE;
+            const uint32_t q_lo = q_lo0 + (g * QBUF + (q_count[g] - 1) % QBUF) * STAGE, k_lo = k_lo0 + ks * STAGE;
             umma_ss<false>(d, q_lo, k_lo, idesc_qk, leader);
 #pragma unroll
             for (int kk = 1; kk < D / 16; kk++)
                 umma_ss<true>(d, q_lo + (kk >> 2) * HALF + 2 * (kk & 3), k_lo + (kk >> 2) * HALF + 2 * (kk & 3), idesc_qk, leader);
             umma_commit_if(s_full + 8 * g, leader);
         };
-        /* the first unit with keys */
-        bool have = false;
-        while (!have && cursor.next(args, u)) have = u.steps != 0;
-        if (have && wait(kv_full + 8 * (tile % RING), (tile / RING) & 1u)) {
+        auto next_unit = [&](uint32_t &steps, bool &second) {
+            steps = 0;
+            while (!steps && cursor.next(args, u)) steps = u.steps;
+            second = GROUPS == 2 && u.rows[1] != 0;
+        };
+        /* steps of this unit and the next, and whether their second tiles have rows */
+        uint32_t steps, n_steps;
+        bool second, n_second;
+        next_unit(steps, second);
+        if (steps && wait(kv_full, 0)) {
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
-                if (!u.rows[g]) continue;
+                if (g && !second) continue;
                 if (!wait(q_full + 8 * (g * QBUF), 0)) break;
                 q_count[g]++;
                 tc_fence_after();
-                issue_qk(g, tile);
+                issue_qk(g, 0);
             }
-            umma_commit_if(kv_free + 8 * (tile % RING), leader);
+            umma_commit_if(kv_free, leader);
         }
-        uint32_t j = 0;
-        while (alive && have) {
-            /* step j of unit u: its V tile is ring position tile + 1, the next step's K tile + 2 */
-            const uint32_t v_tile = tile + 1, k_tile = tile + 2;
-            const bool last = j + 1 == u.steps;
-            CrossUnit n = u;
-            bool more = true;
-            if (last) {
-                more = false;
-                while (!more && cursor.next(args, n)) more = n.steps != 0;
-            }
-            bool k_seen = false, v_seen = false;
+        uint32_t vs = 1 % RING, v_phase = RING == 1, j = 0;      /* ring stage of this step's V tile */
+        if (alive && steps) next_unit(n_steps, n_second);
+        while (alive && steps) {
+            /* Step j: P.V, then the scores of the next step, maybe the next unit's. The loads are waited for
+             * before the probabilities: K's stage was freed by the step before. */
+            const bool last = j + 1 == steps, more = !last || n_steps;
+            const uint32_t ks = vs + 1 == RING ? 0 : vs + 1, k_phase = v_phase ^ (vs + 1 == RING);
+            if (!wait(kv_full + 8 * vs, v_phase)) break;
+            if (more && !wait(kv_full + 8 * ks, k_phase)) break;
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
-                if (alive && u.rows[g]) {
-                    if (!v_seen && !wait(kv_full + 8 * (v_tile % RING), (v_tile / RING) & 1u)) break;
-                    v_seen = true;
-                    if (!wait(p_full + 8 * g, p_count[g] & 1u)) break;
-                    p_count[g]++;
+                if (g == 0 || second) {
+                    if (!wait(p_full + 8 * g, p_phase[g])) break;
+                    p_phase[g] ^= 1;
                     tc_fence_after();
-                    const uint32_t d = tmem_base + COL_O + g * D, a = tmem_base + g * CT;
-                    const uint32_t v_lo = v_lo0 + (v_tile % RING) * STAGE;
+                    const uint32_t d = tmem_base + COL_O + g * D, a = tmem_base + g * CT, v_lo = v_lo0 + vs * STAGE;
                     if (j == 0) umma_ts<false>(d, a, v_lo, idesc_pv, leader);
                     else umma_ts<true>(d, a, v_lo, idesc_pv, leader);
 #pragma unroll
-                    for (uint32_t kk = 1; kk < 8; kk++) umma_ts<true>(d, a + kk * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader);
+                    for (uint32_t kk = 1; kk < 8; kk++)       /* P of keys 64.. lies on the columns of their scores */
+                        umma_ts<true>(d, a + (kk >> 2) * 64 + (kk & 3) * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader);
                     if (last) umma_commit_if(o_done + 8 * g, leader);
                 }
-                if (alive && more && n.rows[g]) {
-                    if (!k_seen && !wait(kv_full + 8 * (k_tile % RING), (k_tile / RING) & 1u)) break;
-                    k_seen = true;
+                if (last ? n_steps && (g == 0 || n_second) : g == 0 || second) {
                     if (last) {
                         if (!wait(q_full + 8 * (g * QBUF + q_count[g] % QBUF), (q_count[g] / QBUF) & 1u)) break;
                         q_count[g]++;
+                        tc_fence_after();
                     }
-                    tc_fence_after();
-                    issue_qk(g, k_tile);
+                    issue_qk(g, ks);
                 }
             }
             if (!alive) break;
-            umma_commit_if(kv_free + 8 * (v_tile % RING), leader);
-            if (more) umma_commit_if(kv_free + 8 * (k_tile % RING), leader);
-            tile += 2;
-            have = more;
-            u = n;
-            j = last ? 0 : j + 1;
+            umma_commit_if(kv_free + 8 * vs, leader);
+            if (more) umma_commit_if(kv_free + 8 * ks, leader);
+            vs = ks + 1 == RING ? 0 : ks + 1;
+            v_phase = k_phase ^ (ks + 1 == RING);
+            j++;
+            if (last) {
+                j = 0;
+                steps = n_steps;
+                second = n_second;
+                if (steps) next_unit(n_steps, n_second);
+            }
         }
     } else {
         /* --------------------------------------------------------------------- softmax */
-        const int g = (warp - 2) >> 2;
-        const uint32_t quarter = warp & 3, local_row = quarter * 32 + lane, lane_base = (quarter * 32) << 16;
-        const uint32_t tmem_s = tmem_base + g * CT + lane_base, tmem_o = tmem_base + COL_O + g * D + lane_base;
+        const int g = (warp - 2) >> 3;
+        const uint32_t half = ((warp - 2) >> 2) & 1, quarter = warp & 3, local_row = quarter * 32 + lane;
+        const uint32_t lane_base = (quarter * 32) << 16;
+        const uint32_t tmem_s = tmem_base + g * CT + half * 64 + lane_base;
+        const uint32_t tmem_o = tmem_base + COL_O + g * D + half * (D / 2) + lane_base;      /* this thread's half of O */
+        const uint32_t pair = 1 + g * 4 + quarter;                                          /* named barrier of a row's two warps */
+        volatile float *my_x = xchg + (g * 2 + half) * CT + local_row, *their_x = xchg + (g * 2 + (half ^ 1)) * CT + local_row;
         const float scale_log2 = args.scale_log2;
         const uint64_t scale2 = pack_f32x2(scale_log2, scale_log2);
-        uint32_t q_count = 0, s_count = 0, o_count = 0, tile = 0;
-        bool alive = true;
-        while (alive && cursor.next(args, u)) {
+        /* the two warps of a row meet; both carry on or neither does */
+        auto meet = [&](bool ok) {
+            uint32_t both;
+            asm volatile("{\n\t.reg .pred pin, pout;\n\tsetp.ne.u32 pin, %2, 0;\n\t"
+                         "bar.red.and.pred pout, %1, 64, pin;\n\tselp.u32 %0, 1, 0, pout;\n\t}"
+                         : "=r"(both) : "r"(pair), "r"(uint32_t(ok)) : "memory");
+            return both != 0;
+        };
+        uint32_t s_phase = 0, o_phase = 0, q_count = 0, tile = 0;
+        bool alive = true, pending = false;
+        /* The unit's query buffer carried its output to the copy engine: it is free once that has been read */
+        auto release_queries = [&] {
+            if (lane == 0 && pending) {
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                mbar_arrive(q_free + 8 * (g * QBUF + (q_count - 1) % QBUF));
+            }
+            pending = false;
+        };
+        bool have = cursor.next(args, u);
+        while (have) {
             const uint32_t rows = g == 0 ? u.rows[0] : u.rows[1];
-            /* this thread's output row */
-            const uint32_t live = (local_row >> args.pack_log2) < rows;
-            const size_t row = size_t(u.q_row + g * (CT >> args.pack_log2) + (local_row >> args.pack_log2));
-            const uint32_t head = u.head0 + (local_row & (args.pack - 1));
-            if (!rows) { tile += 2 * u.steps; continue; }
-            if (!u.steps) {
-                /* no keys: zeros, or a part that weighs nothing */
-                if (live && args.splits == 1) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(args.out + (row * args.heads + head) * D);
+            const uint32_t q_row = u.q_row + g * (CT >> args.pack_log2);          /* of the tile */
+            const uint32_t steps = u.steps;
+            /* (row, head) this thread's accumulators belong to, and whether that row exists */
+            auto unit_of_row = [&] { return size_t(q_row + (local_row >> args.pack_log2)) * args.heads + u.head0 + (local_row & (args.pack - 1)); };
+            const bool live = (local_row >> args.pack_log2) < rows;
+            if (!rows || !steps) {
+                if (live && args.splits == 1) {            /* no keys: zeros */
+                    uint4 *dst = reinterpret_cast<uint4 *>(args.out + unit_of_row() * D + half * (D / 2));
 #pragma unroll
-                    for (int i = 0; i < D / 8; i++) dst[i] = make_uint4(0, 0, 0, 0);
-                } else if (live) {
-                    *reinterpret_cast<float2 *>(args.partial_ml + ((size_t(u.split) * args.query_rows + row) * args.heads + head) * 2) =
+                    for (int i = 0; i < D / 16; i++) dst[i] = make_uint4(0, 0, 0, 0);
+                } else if (live && !half) {                /* a part that weighs nothing */
+                    *reinterpret_cast<float2 *>(args.partial_ml + (size_t(u.split) * args.query_rows * args.heads + unit_of_row()) * 2) =
                         make_float2(-INFINITY, 0.0f);
                 }
+                tile += 2 * steps;
+                have = cursor.next(args, u);
                 continue;
             }
             float reference = -INFINITY, sum = 0.0f;
-            for (uint32_t j = 0; j < u.steps; j++) {
-                alive = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, s_count & 1u, stop, budget));
-                if (!alive) break;
-                s_count++;
+            for (uint32_t j = 0; j < steps; j++) {
+                bool ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, s_phase, stop, budget));
+                s_phase ^= 1;
                 tc_fence_after();
-                const uint32_t valid = u.keys - j * CT;
-                /* GROUPS 2 holds the 128 scores in registers; with two CTAs per SM there is room for 32,
-                 * and they are read from tensor memory twice */
-                uint32_t s[GROUPS == 2 ? CT : 32];
-                float m_step = -INFINITY;
-                auto clip = [&](uint32_t *v, int first, int count) {
-                    if (valid < CT) {
-#pragma unroll
-                        for (int i = 0; i < count; i++)
-                            if (uint32_t(first + i) >= valid) v[i] = 0xff800000u;
-                    }
-                };
-                auto most_of = [&](const uint32_t *v, int count) {
-                    float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < count; i += 4) {
-                        m0 = max3_f32(m0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                        m1 = max3_f32(m1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-                    }
-                    return fmaxf(m0, m1);
-                };
-                if constexpr (GROUPS == 2) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) tmem_ld32(tmem_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                const int valid = int(min(u.keys - j * CT, uint32_t(CT))) - int(half * 64);
+                /* 32 scores at a time, read from tensor memory twice (for the maximum, for the exponentials):
+                 * holding all 64 spills at the 96 registers there are for 18 warps */
+                uint32_t s[32];
+                auto scores = [&](int c) {
+                    tmem_ld32(tmem_s + 32 * c, s);
                     tmem_ld_wait();
-                    clip(s, 0, CT);
-                    m_step = most_of(s, CT);
-                } else {
+                    if (valid < 32 * c + 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (32 * c + i >= valid) s[i] = 0xff800000u;      /* -inf */
+                    }
+                };
+                float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        tmem_ld32(tmem_s + 32 * c, s);
-                        tmem_ld_wait();
-                        clip(s, 32 * c, 32);
-                        m_step = fmaxf(m_step, most_of(s, 32));
+                for (int c = 0; c < 2; c++) {
+                    scores(c);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        m0 = max3_f32(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        m1 = max3_f32(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                        m2 = max3_f32(m2, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
+                        m3 = max3_f32(m3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
                     }
                 }
-                m_step *= scale_log2;
+                float m_step = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+                /* The row's other half. A slot is read before it is written again: these scores imply P.V of the
+                 * step before, which implies that both halves had read theirs. */
+                *my_x = m_step;
+                alive = meet(ok);
+                if (!alive) break;
+                m_step = fmaxf(m_step, *their_x) * scale_log2;
                 const bool raise = m_step - reference > CT_RAISE;      /* true at the first finite score */
                 if (j > 0 && __any_sync(0xffffffffu, raise)) {
                     const float alpha = raise ? ct_exp2(reference - m_step) : 1.0f;
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; c++) {
-                        uint32_t o[32];
-                        tmem_ld32(tmem_o + c * 32, o);
+                    for (int c = 0; c < D / 2; c += 16) {
+                        uint32_t o[16];
+                        ct_ld16(tmem_o + c, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_st32(tmem_o + c * 32, o);
+                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        ct_st16(tmem_o + c, o);
                     }
-                    tmem_st_wait_all();
                 }
                 if (raise) {
                     sum *= ct_exp2(reference - m_step);      /* 0 from -inf */
@@ -507,37 +553,24 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 const float neg_m = reference == -INFINITY ? 0.0f : -reference;
                 const uint64_t neg_m2 = pack_f32x2(neg_m, neg_m);
                 uint64_t sum_a = 0, sum_b = 0;
-                if constexpr (GROUPS == 2) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t packed[16];
-                        ct_exponentials(s + 32 * c, scale2, neg_m2, packed, sum_a, sum_b);
-                        ct_st16(tmem_s + c * 16, packed);
-                    }
-                } else {
-                    /* P chunk c lands on columns 16 c .. 16 c + 15, in front of the scores still to be read */
 #pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t packed[16];
-                        tmem_ld32(tmem_s + 32 * c, s);
-                        tmem_ld_wait();
-                        clip(s, 32 * c, 32);
-                        ct_exponentials(s, scale2, neg_m2, packed, sum_a, sum_b);
-                        ct_st16(tmem_s + c * 16, packed);
-                    }
+                for (int c = 0; c < 2; c++) {
+                    /* P of 32 keys lands on columns in front of the scores that are still to be read */
+                    uint32_t packed[16];
+                    scores(c);
+                    ct_exponentials(s, scale2, neg_m2, packed, sum_a, sum_b);
+                    ct_st16(tmem_s + c * 16, packed);
                 }
-                if (g == 0 && u.dirty && j + 1 == u.steps) {
+                if (g == 0 && u.dirty && j + 1 == steps) {
                     /* value rows that are not the segment's: cleared before anybody's P.V, which is issued
                      * behind this group's arrival */
                     const uint32_t v_tile = tile + 2 * j + 1, stage = v_tile % RING;
-                    alive = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (v_tile / RING) & 1u, stop, budget));
-                    if (!alive) break;
-                    if (local_row >= valid) {
-                        const uint32_t at = ring_smem + stage * TILE + local_row * 128;
+                    ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (v_tile / RING) & 1u, stop, budget));
+                    if (ok && local_row >= u.keys - j * CT) {
+                        const uint32_t at = ring_smem + stage * TILE + local_row * 128 + (D == 128 ? half * CT_BOX : half * 64);
 #pragma unroll
-                        for (int i = 0; i < D / 8; i++)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
-                                         ::"r"(at + (i >> 3) * CT_BOX + (i & 7) * 16), "r"(0) : "memory");
+                        for (int i = 0; i < D / 16; i++)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + i * 16), "r"(0) : "memory");
                     }
                     fence_async_smem();
                 }
@@ -545,79 +578,94 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + 8 * g);
+                if (QBUF == 2 && j == 0) release_queries();
                 float s0, s1, s2, s3;
                 unpack_f32x2(sum_a, s0, s1);
                 unpack_f32x2(sum_b, s2, s3);
                 sum += (s0 + s1) + (s2 + s3);
             }
             if (!alive) break;
-            tile += 2 * u.steps;
-            alive = __all_sync(0xffffffffu, mbar_wait(o_done + 8 * g, o_count & 1u, stop, budget));
+            tile += 2 * steps;
+            /* While P.V runs: the row's sum, through the slots the other way round (each thread writes the one
+             * it has read and reads the one it wrote, so nobody's pending read is overwritten) */
+            *their_x = sum;
+            alive = meet(true);
             if (!alive) break;
-            o_count++;
-            tc_fence_after();
-            const uint32_t q_slot = g * QBUF + q_count % QBUF;
+            sum += *my_x;
             q_count++;
+            const size_t unit = unit_of_row();
+            const uint32_t head0 = u.head0, split = u.split;
+            have = cursor.next(args, u);
+            alive = meet(__all_sync(0xffffffffu, mbar_wait(o_done + 8 * g, o_phase, stop, budget)));
+            if (!alive) break;
+            o_phase ^= 1;
+            tc_fence_after();
             if (args.splits > 1) {
-                const size_t at = (size_t(u.split) * args.query_rows + row) * args.heads + head;
-                if (live) *reinterpret_cast<float2 *>(args.partial_ml + at * 2) = make_float2(reference, sum);
-#pragma unroll 1
-                for (int c = 0; c < D / 32; c++) {
+                const size_t at = size_t(split) * args.query_rows * args.heads + unit;
+                if (live && !half) *reinterpret_cast<float2 *>(args.partial_ml + at * 2) = make_float2(reference, sum);
+#pragma unroll
+                for (int c = 0; c < D / 2; c += 32) {
                     uint32_t o[32];
-                    tmem_ld32(tmem_o + c * 32, o);
+                    tmem_ld32(tmem_o + c, o);
                     tmem_ld_wait();
                     if (live) {
 #pragma unroll
                         for (int i = 0; i < 8; i++)
-                            reinterpret_cast<uint4 *>(args.partial_o + at * D + c * 32)[i] =
+                            reinterpret_cast<uint4 *>(args.partial_o + at * D + half * (D / 2) + c)[i] =
                                 make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
+                if (lane == 0) mbar_arrive(q_free + 8 * (g * QBUF + (q_count - 1) % QBUF));
             } else {
-                /* all scores -inf: zeros; a NaN sum stays NaN */
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                /* the tile's queries are not needed any more: their buffer turns rows held by threads into
-                 * whole-row stores (16-byte pieces, XOR-swizzled by row) */
-                constexpr uint32_t ROW_BYTES = D * 2, CHUNKS = D / 8, ROWS_PER_STORE = 32 / CHUNKS;
-                const uint32_t stage = q_smem + q_slot * TILE + quarter * 32 * ROW_BYTES;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; c++) {
-                    uint32_t o[32];
-                    tmem_ld32(tmem_o + c * 32, o);
+                /* All scores -inf: zeros; a NaN sum stays NaN. A whole tile goes through the tile's query buffer
+                 * (its scores are complete) to the copy engine, 32 rows x D / 2 dims per warp: 32 KiB stored
+                 * row by row would cost the shared-memory path a cycle per 16 or 32 bytes, and the tensor
+                 * core reads its operands through the same path. */
+                const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
+                const bool whole = rows == (CT >> args.pack_log2) && args.block_stores;
+                const uint32_t buffer = q_smem + (g * QBUF + (q_count - 1) % QBUF) * TILE + (D == 128 ? half * CT_BOX : 0);
+                const uint32_t line = buffer + local_row * 128, turn = local_row & 7;
+#pragma unroll
+                for (int c = 0; c < D / 2; c += 32) {
+                    uint32_t o[32], packed[16];
+                    tmem_ld32(tmem_o + c, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (uint32_t v = 0; v < 4; v++) {
-                        const uint32_t at = stage + lane * ROW_BYTES + (((c * 4 + v) ^ (lane & (CHUNKS - 1))) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
-                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv)),
-                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv)),
-                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv)),
-                                     "r"(pack_bf16(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv))
-                                     : "memory");
-                    }
-                }
-                __syncwarp();
-                const uint32_t chunk = lane & (CHUNKS - 1);
+                    for (int i = 0; i < 16; i++)
+                        packed[i] = pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    if (whole) {
 #pragma unroll
-                for (uint32_t i = 0; i < CHUNKS; i++) {
-                    const uint32_t r = ROWS_PER_STORE * i + lane / CHUNKS, t = quarter * 32 + r;
-                    uint4 val;
-                    const uint32_t at = stage + r * ROW_BYTES + ((chunk ^ (r & (CHUNKS - 1))) << 4);
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(val.x), "=r"(val.y), "=r"(val.z), "=r"(val.w) : "r"(at) : "memory");
-                    if ((t >> args.pack_log2) < rows) {
-                        const size_t out_row = size_t(u.q_row + g * (CT >> args.pack_log2) + (t >> args.pack_log2));
-                        *reinterpret_cast<uint4 *>(args.out + (out_row * args.heads + u.head0 + (t & (args.pack - 1))) * D + chunk * 8) = val;
+                        for (uint32_t i = 0; i < 4; i++) {
+                            const uint32_t chunk = (D == 128 ? 0 : half * 4) + c / 8 + i;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((chunk ^ turn) << 4)),
+                                         "r"(packed[4 * i]), "r"(packed[4 * i + 1]), "r"(packed[4 * i + 2]), "r"(packed[4 * i + 3]) : "memory");
+                        }
+                    } else if (live) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            reinterpret_cast<uint4 *>(args.out + unit * D + half * (D / 2) + c)[i] =
+                                make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
                     }
                 }
-                fence_async_smem();
+                if (whole) {
+                    fence_async_smem();
+                    /* 64-dim lines: with head_dim 64 the two warps of a row fill one line together */
+                    if (D == 64) meet(true);
+                    __syncwarp();
+                    if (lane == 0 && (D == 128 || half == 0)) {
+                        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                                     ::"l"(&map_out), "r"(buffer + quarter * 32 * 128), "r"(D == 128 ? int(half * 64) : 0), "r"(int(head0)),
+                                       "r"(int(q_row + (quarter * 32 >> args.pack_log2))) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+                pending = true;
+                if (QBUF == 1 || !have) release_queries();
             }
-            /* O has been read and the query buffer is done with: the next unit's P.V waits for this group's
-             * next P anyway, the next queries for this */
+            /* O has been read: the next unit's P.V waits for this group's next P */
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_free + 8 * q_slot);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     __syncwarp();
@@ -706,8 +754,12 @@ bool ct_configure(int device) {
 template <int D, int GROUPS>
 int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k, const uint16_t *v) {
     if (!ct_configure<D, GROUPS>(gpu->device)) return h3b_fail(gpu, "cannot reserve shared memory for the cross attention kernel");
-    CUtensorMap map_q, map_k, map_v;
-    if (!ct_map(&map_q, q, args.query_rows, args.heads, D, args.pack, CT >> args.pack_log2) ||
+    CUtensorMap map_q, map_k, map_v, map_out;
+    /* a warp's block of the output is 32 tile rows */
+    args.block_stores = args.pack <= 32;
+    if (!ct_map(&map_out, args.out, args.query_rows, args.heads, D, args.block_stores ? args.pack : 1,
+                args.block_stores ? 32 >> args.pack_log2 : 32) ||
+        !ct_map(&map_q, q, args.query_rows, args.heads, D, args.pack, CT >> args.pack_log2) ||
         !ct_map(&map_k, k, args.key_rows, args.kv_heads, D, 1, CT) || !ct_map(&map_v, v, args.key_rows, args.kv_heads, D, 1, CT))
         return h3b_fail(gpu, "cannot encode the cross attention tensor maps");
     /* most units there can be: every segment may end in a part of a tile */
@@ -716,13 +768,16 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
     if (units > 0xffffffffull - gpu->sm_count * 2) return h3b_fail(gpu, "cross attention has too many tiles");
     const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2);
     const unsigned grid = unsigned(units < resident ? units : resident);
+    args.step_h = grid % args.head_units;
+    args.step_s = grid / args.head_units % args.splits;
+    args.step_i = grid / args.head_units / args.splits;
     h3b_scratch scratch(gpu, args.splits > 1 ? size_t(args.splits) * args.query_rows * args.heads * (D + 2) * sizeof(float) : 0);
     if (args.splits > 1) {
         if (!scratch.data) return h3b_fail(gpu, "cross_sdpa_bf16: cannot allocate the partial results");
         args.partial_o = static_cast<float *>(scratch.data);
         args.partial_ml = args.partial_o + size_t(args.splits) * args.query_rows * args.heads * D;
     }
-    h3b_cross_tc<D, GROUPS><<<grid, ct_threads<GROUPS>(), ct_smem<D, GROUPS>(), gpu->stream>>>(map_q, map_k, map_v, args);
+    h3b_cross_tc<D, GROUPS><<<grid, ct_threads<GROUPS>(), ct_smem<D, GROUPS>(), gpu->stream>>>(map_q, map_k, map_v, map_out, args);
     if (args.splits > 1) {
         const size_t warps = size_t(args.query_rows) * args.heads;
         h3b_cross_merge<D><<<unsigned((warps + 7) / 8), 256, 0, gpu->stream>>>(args);
@@ -786,6 +841,7 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
         while (args.pack_log2 < 7 && group % (2u << args.pack_log2) == 0) args.pack_log2++;
         args.pack = 1u << args.pack_log2;
         args.head_units = heads / args.pack;
+        args.units_per_kv = group / args.pack;
         args.scale_log2 = scale * 1.4426950408889634f;
         const bool few = query_rows <= uint64_t(segment_count) * (CT >> args.pack_log2);
         args.splits = 1;
