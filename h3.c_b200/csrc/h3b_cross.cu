@@ -12,6 +12,7 @@
 
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 namespace {
 
@@ -116,15 +117,21 @@ h3b_cross_simt(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t
  * A query tile is 128 rows of tensor memory: 128 / pack query rows of `pack` neighbouring heads that
  * share a key head (pack = the largest power of two in heads / kv_heads), so that shared key heads are
  * read once per tile. A work unit is GROUPS neighbouring tiles of one segment and head set over a range of
- * 128-key tiles; one persistent CTA per SM (GROUPS 2) walks units w, w + grid, ...
+ * 128-key tiles ("steps"); persistent CTAs walk units w, w + grid, ... The steps of all units of a CTA
+ * count on in t: t names buffers and barrier phases, and step t + 1 may be the next unit's first.
  *
- *   warp 0   TMA: the unit's query tiles into one of QBUF buffers per group, K and V tiles through one
- *            ring in the order K0 V0 K1 V1 ..., shared by the groups.
- *   warp 1   tcgen05.mma: per step and group O += P.V, then the group's next scores Q.K^T. The next
- *            step may belong to the next unit, so the tensor pipe never drains between units: states
- *            are short (one to four steps), and a CTA per tile spends half of its time filling and
- *            draining. P (BF16) overwrites the scores it came from and is the A operand of P.V; the
- *            in-order pipe keeps the next scores behind it.
+ *   warp 0   TMA. Stage t % STAGES holds what the tensor core reads after the softmax of step t: V(t) and
+ *            K(t + 1). With a unit's last step come the next unit's queries (one buffer per group: the
+ *            scores of the last step have been computed by then).
+ *   warp 1   tcgen05.mma, per step and group: O += P(t).V(t), then the group's scores Q.K(t + 1)^T. The tensor
+ *            pipe does not drain between units: states are short (one to four steps), and a CTA per
+ *            tile would spend half of its time filling and draining. All the group waits for collects on
+ *            one barrier, go[group][t % 2]: the softmax warps' arrivals for P(t) and, for the first group, the
+ *            bytes of V(t) and K(t + 1). Behind a unit's last P.V come the scores of the next unit, once its
+ *            queries are there (the groups write their outputs meanwhile). The issuing warp is one instruction stream of 4 to 5 cycles an
+ *            instruction: with a barrier each for P, K, V and Q it needed 3,270 cycles per step of two
+ *            groups without a single MMA. P (BF16) overwrites the scores it came from and is the A
+ *            operand of P.V; the in-order pipe keeps the next scores behind it.
  *   warps 2+ softmax, 8 warps per group: two threads own a row, each 64 of a step's 128 keys and half of
  *            the output; they exchange their maxima through shared memory and a named barrier of their
  *            two warps, which also carries the vote to go on. Scores of a step complete imply that
@@ -139,13 +146,14 @@ constexpr int CT_BOX = CT * 64 * 2;                  /* a TMA box: 128 rows x 64
 constexpr float CT_RAISE = 8.0f;                     /* raise the reference by more than 2^8 only */
 
 template <int D> constexpr int ct_tile() { return CT * D * 2; }
-template <int D, int GROUPS> constexpr int ct_qbuf() { return GROUPS == 2 ? 2 : 1; }
-template <int D, int GROUPS> constexpr int ct_ring() { return GROUPS == 2 ? (D == 128 ? 3 : 8) : (D == 128 ? 2 : 4); }
+template <int GROUPS> constexpr int ct_stages() { return GROUPS; }
 template <int GROUPS> constexpr int ct_threads() { return 64 + 256 * GROUPS; }
-constexpr int CT_BARS = 512;
+constexpr int CT_BARS = 256;
+constexpr int CT_OUT = 32 * 64;                      /* output staging of a warp: 32 rows x 32 dims */
+template <int GROUPS> constexpr int ct_out() { return GROUPS == 2 ? GROUPS * 8 * CT_OUT : 0; }
 template <int GROUPS> constexpr int ct_xchg() { return GROUPS * 2 * CT * 4; }    /* [group][half][row] */
 template <int D, int GROUPS> constexpr size_t ct_smem() {
-    return size_t(GROUPS * ct_qbuf<D, GROUPS>() + ct_ring<D, GROUPS>()) * ct_tile<D>() + CT_BARS + ct_xchg<GROUPS>();
+    return size_t(GROUPS + 2 * ct_stages<GROUPS>()) * ct_tile<D>() + ct_out<GROUPS>() + CT_BARS + ct_xchg<GROUPS>();
 }
 static_assert(ct_smem<128, 2>() <= 232448, "cross attention needs at most 227 KiB of shared memory");
 static_assert(2 * (ct_smem<128, 1>() + 1024) <= 233472, "two one-group CTAs per SM");
@@ -167,7 +175,7 @@ struct CrossArgs {
 
 /* One work unit; every role walks the same units with a cursor of its own */
 struct CrossUnit {
-    uint32_t q_row, rows[2];     /* first query row; live query rows of each group's tile */
+    uint32_t q_row, rows;        /* first query row, live query rows (of all groups) */
     uint32_t head0, kv_head;
     uint32_t k_row, keys;        /* first key row of the range; keys of the segment from there on */
     uint32_t steps, split;
@@ -199,8 +207,7 @@ struct CrossCursor {
         }
         const uint32_t tile_rows = CT >> a.pack_log2, first = (item - before) * GROUPS * tile_rows, left = segment.queries - first;
         u.q_row = segment.q0 + first;
-        u.rows[0] = min(tile_rows, left);
-        u.rows[1] = GROUPS == 2 && left > tile_rows ? min(tile_rows, left - tile_rows) : 0;
+        u.rows = min(GROUPS * tile_rows, left);
         u.head0 = h << a.pack_log2;
         u.kv_head = a.units_per_kv == 1 ? h : h / a.units_per_kv;
         u.split = s;
@@ -272,21 +279,23 @@ __global__ void __launch_bounds__(ct_threads<GROUPS>(), GROUPS == 2 ? 1 : 2)
 h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
              const __grid_constant__ CrossArgs args) {
-    constexpr int TILE = ct_tile<D>(), QBUF = ct_qbuf<D, GROUPS>(), RING = ct_ring<D, GROUPS>();
+    constexpr int TILE = ct_tile<D>(), STAGES = ct_stages<GROUPS>();
     constexpr uint32_t COL_O = GROUPS * CT, TMEM_COLS = GROUPS * 256;
     extern __shared__ __align__(1024) uint8_t ct_smem_raw[];
     const uint32_t base = smem_u32(ct_smem_raw);
-    const uint32_t q_smem = base;                                   /* [group][buffer] */
-    const uint32_t ring_smem = q_smem + GROUPS * QBUF * TILE;
-    const uint32_t bars = ring_smem + RING * TILE;
-    const uint32_t q_full = bars;                                   /* [group][buffer] = 4 */
-    const uint32_t q_free = q_full + 32;                            /* [group][buffer] = 4 */
-    const uint32_t kv_full = q_free + 32;                           /* [stage] = 8         */
-    const uint32_t kv_free = kv_full + 64;                          /* [stage] = 8         */
-    const uint32_t s_full = kv_free + 64;                           /* [group]             */
-    const uint32_t p_full = s_full + 16;                            /* [group]             */
-    const uint32_t o_done = p_full + 16;                            /* [group]             */
-    const uint32_t holder = o_done + 16;
+    const uint32_t q_smem = base;                                   /* [group]               */
+    const uint32_t k_smem = q_smem + GROUPS * TILE;                 /* [stage]               */
+    const uint32_t v_smem = k_smem + STAGES * TILE;                 /* [stage]               */
+    const uint32_t out_smem = v_smem + STAGES * TILE;               /* [softmax warp]        */
+    const uint32_t bars = out_smem + ct_out<GROUPS>();
+    const uint32_t first = bars;                                    /* K(0)                  */
+    const uint32_t queries = first + 8;                             /* a unit's query tiles  */
+    const uint32_t go = queries + 8;                                /* [group][step % 2] = 4 */
+    const uint32_t s_full = go + 32;                                /* [group] = 2: scores   */
+    const uint32_t o_done = s_full + 16;                            /* [group] = 2           */
+    const uint32_t seen = o_done + 16;                              /* [step % 2]: scores of all groups seen complete */
+    const uint32_t tail = seen + 16;                                /* [step % 2]: V tile that has to be cleared in part */
+    const uint32_t holder = tail + 16;
     volatile int *stop = reinterpret_cast<volatile int *>(ct_smem_raw + (holder + 8 - base));
     volatile float *xchg = reinterpret_cast<volatile float *>(ct_smem_raw + (bars - base) + CT_BARS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -297,11 +306,12 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     }
     if (threadIdx.x == 0) {
         *stop = 0;
-        for (int i = 0; i < GROUPS * QBUF; i++) { mbar_init(q_full + 8 * i, 1); mbar_init(q_free + 8 * i, 8); }
-        for (int i = 0; i < RING; i++) { mbar_init(kv_full + 8 * i, 1); mbar_init(kv_free + 8 * i, 1); }
+        mbar_init(first, 1);
+        mbar_init(queries, 1);
+        for (int i = 0; i < 2 * GROUPS; i++) mbar_init(go + 8 * i, i < 2 ? 9 : 8);      /* 8 softmax warps, the producer */
+        for (int i = 0; i < 2; i++) { mbar_init(seen + 8 * i, 1); mbar_init(tail + 8 * i, 1); }
         for (int g = 0; g < GROUPS; g++) {
             mbar_init(s_full + 8 * g, 1);
-            mbar_init(p_full + 8 * g, 8);
             mbar_init(o_done + 8 * g, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -322,38 +332,64 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     if (warp == 0) {
         /* ---------------------------------------------------------------- TMA producer */
         if (lane == 0) {
-            uint32_t q_count[2] = {0, 0}, stage = 0, round = 0;
-            bool alive = true;
-            /* the K or V tile at key row `row` into the next ring stage */
-            auto load_tile = [&](const CUtensorMap *map, uint32_t row) {
-                if (round && !mbar_wait(kv_free + 8 * stage, (round - 1) & 1u, stop, budget)) return false;
-                const uint32_t bar = kv_full + 8 * stage, dst = ring_smem + stage * TILE;
-                mbar_expect_tx(bar, TILE);
-                ct_load(dst, map, bar, 0, int(u.kv_head), int(row));
-                if (D == 128) ct_load(dst + CT_BOX, map, bar, 64, int(u.kv_head), int(row));
-                if (++stage == RING) { stage = 0; round++; }
-                return true;
+            auto load = [&](const CUtensorMap *map, uint32_t bar, uint32_t dst, uint32_t head, uint32_t row) {
+                ct_load(dst, map, bar, 0, int(head), int(row));
+                if (D == 128) ct_load(dst + CT_BOX, map, bar, 64, int(head), int(row));
             };
-            while (alive && cursor.next(args, u)) {
-                if (!u.steps) continue;
-                alive = load_tile(&map_k, u.k_row);      /* in front of the queries: the MMA warp waits for it first */
-#pragma unroll
-                for (int g = 0; g < GROUPS; g++) {
-                    if (!alive || !u.rows[g]) continue;
-                    const uint32_t buffer = q_count[g] % QBUF, q_round = q_count[g] / QBUF;
-                    alive = !q_round || mbar_wait(q_free + 8 * (g * QBUF + buffer), (q_round - 1) & 1u, stop, budget);
-                    if (!alive) break;
-                    const uint32_t bar = q_full + 8 * (g * QBUF + buffer), dst = q_smem + (g * QBUF + buffer) * TILE;
-                    const int row = int(u.q_row + g * (CT >> args.pack_log2));
-                    mbar_expect_tx(bar, TILE);
-                    ct_load(dst, &map_q, bar, 0, int(u.head0), row);
-                    if (D == 128) ct_load(dst + CT_BOX, &map_q, bar, 64, int(u.head0), row);
-                    q_count[g]++;
+            auto next_unit = [&](CrossUnit &n) {
+                while (cursor.next(args, n))
+                    if (n.steps) return true;
+                return false;
+            };
+            CrossUnit n = {};
+            uint32_t t = 0;
+            bool have = next_unit(u), alive = true;
+            if (have) {
+                mbar_expect_tx(queries, GROUPS * TILE);
+                for (int g = 0; g < GROUPS; g++)
+                    load(&map_q, queries, q_smem + g * TILE, u.head0, u.q_row + g * (CT >> args.pack_log2));
+                mbar_expect_tx(first, TILE);
+                load(&map_k, first, k_smem + (STAGES - 1) * TILE, u.kv_head, u.k_row);
+            }
+            /* has step `e`'s "all scores seen" been waited for? (every one is, in order) */
+            uint32_t events = 0;
+            auto scores_seen = [&](uint32_t e) {
+                while (alive && events <= e) {
+                    alive = mbar_wait(seen + 8 * (events & 1u), (events >> 1) & 1u, stop, budget);
+                    events++;
                 }
-                for (uint32_t j = 0; alive && j < u.steps; j++) {
-                    if (j) alive = load_tile(&map_k, u.k_row + j * CT);
-                    alive = alive && load_tile(&map_v, u.k_row + j * CT);
+                return alive;
+            };
+            while (have && alive) {
+                const bool more = next_unit(n);
+                /* into L2 by the time the single query buffers are free: from memory the load would take longer
+                 * than the last softmax hides (2,800 cycles measured, against 1,000) */
+                for (int g = 0; more && g < GROUPS; g++)
+                    for (int box = 0; box < D / 64; box++)
+                        asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];"
+                                     ::"l"(&map_q), "r"(box * 64), "r"(int(n.head0)), "r"(int(n.q_row + g * (CT >> args.pack_log2))) : "memory");
+                for (uint32_t j = 0; j < u.steps; j++, t++) {
+                    const bool last = j + 1 == u.steps, dirty = last && u.dirty;
+                    /* V(t), K(t + 1) into their stage: V(t - STAGES) and K(t + 1 - STAGES) are dead when the scores
+                     * of step t + 1 - STAGES are complete */
+                    if (t + 1 >= uint32_t(STAGES) && !scores_seen(t + 1 - STAGES)) break;
+                    const uint32_t stage = t % STAGES, bar = go + 8 * (t & 1u);
+                    const bool next_k = !last || more;
+                    mbar_expect_tx(bar, (dirty ? 0 : TILE) + (next_k ? TILE : 0));
+                    if (dirty) mbar_expect_tx(tail + 8 * (t & 1u), TILE);
+                    if (next_k)
+                        load(&map_k, bar, k_smem + stage * TILE, last ? n.kv_head : u.kv_head, last ? n.k_row : u.k_row + (j + 1) * CT);
+                    load(&map_v, dirty ? tail + 8 * (t & 1u) : bar, v_smem + stage * TILE, u.kv_head, u.k_row + j * CT);
+                    if (last && more) {
+                        /* the next queries: their buffers are free when the last scores are complete */
+                        if (!scores_seen(t)) break;
+                        mbar_expect_tx(queries, GROUPS * TILE);
+                        for (int g = 0; g < GROUPS; g++)
+                            load(&map_q, queries, q_smem + g * TILE, n.head0, n.q_row + g * (CT >> args.pack_log2));
+                    }
                 }
+                u = n;
+                have = more;
             }
         }
     } else if (warp == 1) {
@@ -362,88 +398,88 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         constexpr uint32_t idesc_qk = instruction_desc(CT, CT);
         constexpr uint32_t idesc_pv = instruction_desc(CT, D) | (1u << 16);     /* V is N-major */
         constexpr uint32_t HALF = CT_BOX >> 4, STAGE = TILE >> 4;
-        const uint32_t q_lo0 = desc_lo_kmajor(q_smem), k_lo0 = desc_lo_kmajor(ring_smem);
-        const uint32_t v_lo0 = desc_lo_nmajor(ring_smem, CT_BOX);
-        uint32_t q_count[2] = {0, 0}, p_phase[2] = {0, 0};
-        bool alive = true;
+        const uint32_t q_lo0 = desc_lo_kmajor(q_smem), k_lo0 = desc_lo_kmajor(k_smem);
+        const uint32_t v_lo0 = desc_lo_nmajor(v_smem, CT_BOX);
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, budget));
-            return alive;
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, budget));
         };
-        /* scores of group g against the K tile in ring stage `ks`; q_count was advanced at the unit's first step */
-        auto issue_qk = [&](int g, uint32_t ks) {
-            const uint32_t d = tmem_base + g * CT;
-            const uint32_t q_lo = q_lo0 + (g * QBUF + (q_count[g] - 1) % QBUF) * STAGE, k_lo = k_lo0 + ks * STAGE;
-            umma_ss<false>(d, q_lo, k_lo, idesc_qk, leader);
+        using std::integral_constant;
+        /* instructions FROM .. TO - 1 of the D / 16 of a group's scores against the K tile of a stage */
+        auto issue_qk = [&](auto g_const, auto stage_const, auto from_const, auto to_const) {
+            constexpr int g = decltype(g_const)::value, from = decltype(from_const)::value, to = decltype(to_const)::value;
+            const uint32_t d = tmem_base + g * CT, q_lo = q_lo0 + g * STAGE, k_lo = k_lo0 + decltype(stage_const)::value * STAGE;
 #pragma unroll
-            for (int kk = 1; kk < D / 16; kk++)
-                umma_ss<true>(d, q_lo + (kk >> 2) * HALF + 2 * (kk & 3), k_lo + (kk >> 2) * HALF + 2 * (kk & 3), idesc_qk, leader);
-            umma_commit_if(s_full + 8 * g, leader);
+            for (int kk = from; kk < to; kk++) {
+                if (kk == 0) umma_ss<false>(d, q_lo, k_lo, idesc_qk, leader);
+                else umma_ss<true>(d, q_lo + (kk >> 2) * HALF + 2 * (kk & 3), k_lo + (kk >> 2) * HALF + 2 * (kk & 3), idesc_qk, leader);
+            }
+            if (to == D / 16) umma_commit_if(s_full + 8 * g, leader);
         };
-        auto next_unit = [&](uint32_t &steps, bool &second) {
-            steps = 0;
+        auto next_unit = [&] {
+            uint32_t steps = 0;
             while (!steps && cursor.next(args, u)) steps = u.steps;
-            second = GROUPS == 2 && u.rows[1] != 0;
+            return steps;
         };
-        /* steps of this unit and the next, and whether their second tiles have rows */
-        uint32_t steps, n_steps;
-        bool second, n_second;
-        next_unit(steps, second);
-        if (steps && wait(kv_full, 0)) {
-#pragma unroll
-            for (int g = 0; g < GROUPS; g++) {
-                if (g && !second) continue;
-                if (!wait(q_full + 8 * (g * QBUF), 0)) break;
-                q_count[g]++;
-                tc_fence_after();
-                issue_qk(g, 0);
-            }
-            umma_commit_if(kv_free, leader);
+        constexpr integral_constant<int, 0> zero{};
+        constexpr integral_constant<int, D / 16 - 2> most{};
+        constexpr integral_constant<int, D / 16> all{};
+        /* steps left of this unit (this one included) and steps of the next */
+        uint32_t left = next_unit(), n_steps = 0;
+        uint32_t q_phase = 0;
+        bool going = left && wait(first, 0) && wait(queries, 0);
+        if (going) {
+            tc_fence_after();
+            issue_qk(zero, integral_constant<int, STAGES - 1>{}, zero, all);
+            if constexpr (GROUPS == 2) issue_qk(integral_constant<int, 1>{}, integral_constant<int, STAGES - 1>{}, zero, all);
+            q_phase = 1;
+            n_steps = next_unit();
         }
-        uint32_t vs = 1 % RING, v_phase = RING == 1, j = 0;      /* ring stage of this step's V tile */
-        if (alive && steps) next_unit(n_steps, n_second);
-        while (alive && steps) {
-            /* Step j: P.V, then the scores of the next step, maybe the next unit's. The loads are waited for
-             * before the probabilities: K's stage was freed by the step before. */
-            const bool last = j + 1 == steps, more = !last || n_steps;
-            const uint32_t ks = vs + 1 == RING ? 0 : vs + 1, k_phase = v_phase ^ (vs + 1 == RING);
-            if (!wait(kv_full + 8 * vs, v_phase)) break;
-            if (more && !wait(kv_full + 8 * ks, k_phase)) break;
+        /* Unrolled by the step's parity, so that descriptors and barrier addresses are constants; the
+         * barrier that comes next is tested between two MMAs, where that hides behind the pipe. */
+        uint32_t phase = 0, ready = 0, start = 1;      /* start: the unit's first step, which overwrites O */
+        auto step = [&](auto parity_const) {
+            constexpr int PARITY = decltype(parity_const)::value;
+            constexpr integral_constant<int, PARITY % STAGES> stage{};
+            const bool last = left == 1;
+            auto group = [&](auto g_const) {
+                constexpr int g = decltype(g_const)::value;
+                if (!__all_sync(0xffffffffu, ready != 0u) && !wait(go + 16 * g + 8 * PARITY, phase)) return false;
+                tc_fence_after();
+                const uint32_t d = tmem_base + COL_O + g * D, a = tmem_base + g * CT, v_lo = v_lo0 + stage.value * STAGE;
+                if (start) umma_ts<false>(d, a, v_lo, idesc_pv, leader);
+                else umma_ts<true>(d, a, v_lo, idesc_pv, leader);
 #pragma unroll
-            for (int g = 0; g < GROUPS; g++) {
-                if (g == 0 || second) {
-                    if (!wait(p_full + 8 * g, p_phase[g])) break;
-                    p_phase[g] ^= 1;
-                    tc_fence_after();
-                    const uint32_t d = tmem_base + COL_O + g * D, a = tmem_base + g * CT, v_lo = v_lo0 + vs * STAGE;
-                    if (j == 0) umma_ts<false>(d, a, v_lo, idesc_pv, leader);
-                    else umma_ts<true>(d, a, v_lo, idesc_pv, leader);
-#pragma unroll
-                    for (uint32_t kk = 1; kk < 8; kk++)       /* P of keys 64.. lies on the columns of their scores */
-                        umma_ts<true>(d, a + (kk >> 2) * 64 + (kk & 3) * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader);
-                    if (last) umma_commit_if(o_done + 8 * g, leader);
-                }
-                if (last ? n_steps && (g == 0 || n_second) : g == 0 || second) {
-                    if (last) {
-                        if (!wait(q_full + 8 * (g * QBUF + q_count[g] % QBUF), (q_count[g] / QBUF) & 1u)) break;
-                        q_count[g]++;
-                        tc_fence_after();
-                    }
-                    issue_qk(g, ks);
-                }
-            }
-            if (!alive) break;
-            umma_commit_if(kv_free + 8 * vs, leader);
-            if (more) umma_commit_if(kv_free + 8 * ks, leader);
-            vs = ks + 1 == RING ? 0 : ks + 1;
-            v_phase = k_phase ^ (ks + 1 == RING);
-            j++;
+                for (uint32_t kk = 1; kk < 8; kk++)       /* P of keys 64.. lies on the columns of their scores */
+                    umma_ts<true>(d, a + (kk >> 2) * 64 + (kk & 3) * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader);
+                if (last) umma_commit_if(o_done + 8 * g, leader);
+                else issue_qk(g_const, stage, zero, most);
+                if (g + 1 < GROUPS) ready = mbar_test(go + 16 + 8 * PARITY, phase);
+                else ready = mbar_test(go + 8 * (PARITY ^ 1), phase ^ PARITY);
+                if (!last) issue_qk(g_const, stage, most, all);
+                return true;
+            };
+            if (!group(integral_constant<int, 0>{})) return false;
+            if constexpr (GROUPS == 2)
+                if (!group(integral_constant<int, 1>{})) return false;
+            start = last;
+            left--;
             if (last) {
-                j = 0;
-                steps = n_steps;
-                second = n_second;
-                if (steps) next_unit(n_steps, n_second);
+                left = n_steps;
+                if (left) {
+                    if (!wait(queries, q_phase)) return false;
+                    q_phase ^= 1;
+                    tc_fence_after();
+                    issue_qk(zero, stage, zero, all);
+                    if constexpr (GROUPS == 2) issue_qk(integral_constant<int, 1>{}, stage, zero, all);
+                    n_steps = next_unit();
+                }
             }
+            return left != 0;
+        };
+        while (going) {
+            going = step(zero);
+            if (going) going = step(integral_constant<int, 1>{});
+            phase ^= 1;
         }
     } else {
         /* --------------------------------------------------------------------- softmax */
@@ -464,25 +500,17 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                          : "=r"(both) : "r"(pair), "r"(uint32_t(ok)) : "memory");
             return both != 0;
         };
-        uint32_t s_phase = 0, o_phase = 0, q_count = 0, tile = 0;
-        bool alive = true, pending = false;
-        /* The unit's query buffer carried its output to the copy engine: it is free once that has been read */
-        auto release_queries = [&] {
-            if (lane == 0 && pending) {
-                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                mbar_arrive(q_free + 8 * (g * QBUF + (q_count - 1) % QBUF));
-            }
-            pending = false;
-        };
+        uint32_t t = 0, o_phase = 0, tail_phase = 0;
+        bool alive = true;
         bool have = cursor.next(args, u);
         while (have) {
-            const uint32_t rows = g == 0 ? u.rows[0] : u.rows[1];
-            const uint32_t q_row = u.q_row + g * (CT >> args.pack_log2);          /* of the tile */
+            const uint32_t tile_rows = CT >> args.pack_log2, row_in_tile = local_row >> args.pack_log2;
+            const uint32_t q_row = u.q_row + g * tile_rows;                       /* of the tile */
+            const bool live = g * tile_rows + row_in_tile < u.rows, whole = (g + 1) * tile_rows <= u.rows;
+            /* (row, head) this thread's accumulators belong to */
+            auto unit_of_row = [&] { return size_t(q_row + row_in_tile) * args.heads + u.head0 + (local_row & (args.pack - 1)); };
             const uint32_t steps = u.steps;
-            /* (row, head) this thread's accumulators belong to, and whether that row exists */
-            auto unit_of_row = [&] { return size_t(q_row + (local_row >> args.pack_log2)) * args.heads + u.head0 + (local_row & (args.pack - 1)); };
-            const bool live = (local_row >> args.pack_log2) < rows;
-            if (!rows || !steps) {
+            if (!steps) {
                 if (live && args.splits == 1) {            /* no keys: zeros */
                     uint4 *dst = reinterpret_cast<uint4 *>(args.out + unit_of_row() * D + half * (D / 2));
 #pragma unroll
@@ -491,15 +519,15 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     *reinterpret_cast<float2 *>(args.partial_ml + (size_t(u.split) * args.query_rows * args.heads + unit_of_row()) * 2) =
                         make_float2(-INFINITY, 0.0f);
                 }
-                tile += 2 * steps;
                 have = cursor.next(args, u);
                 continue;
             }
             float reference = -INFINITY, sum = 0.0f;
-            for (uint32_t j = 0; j < steps; j++) {
-                bool ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, s_phase, stop, budget));
-                s_phase ^= 1;
+            for (uint32_t j = 0; j < steps; j++, t++) {
+                bool ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, t & 1u, stop, budget));
                 tc_fence_after();
+                /* the last group's scores are the last to be complete: the stage before is free */
+                if (g == GROUPS - 1 && half == 0 && quarter == 0 && lane == 0) mbar_arrive(seen + 8 * (t & 1u));
                 const int valid = int(min(u.keys - j * CT, uint32_t(CT))) - int(half * 64);
                 /* 32 scores at a time, read from tensor memory twice (for the maximum, for the exponentials):
                  * holding all 64 spills at the 96 registers there are for 18 warps */
@@ -514,8 +542,8 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     }
                 };
                 float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int c = 1; c >= 0; c--) {       /* the first 32 stay in registers */
                     scores(c);
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
@@ -553,46 +581,43 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 const float neg_m = reference == -INFINITY ? 0.0f : -reference;
                 const uint64_t neg_m2 = pack_f32x2(neg_m, neg_m);
                 uint64_t sum_a = 0, sum_b = 0;
-#pragma unroll 1
+                /* P of 32 keys lands on columns in front of the scores that are still to be read */
+#pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    /* P of 32 keys lands on columns in front of the scores that are still to be read */
                     uint32_t packed[16];
-                    scores(c);
+                    if (c) scores(c);
                     ct_exponentials(s, scale2, neg_m2, packed, sum_a, sum_b);
                     ct_st16(tmem_s + c * 16, packed);
                 }
-                if (g == 0 && u.dirty && j + 1 == steps) {
+                if (u.dirty && j + 1 == steps && g == 0) {
                     /* value rows that are not the segment's: cleared before anybody's P.V, which is issued
                      * behind this group's arrival */
-                    const uint32_t v_tile = tile + 2 * j + 1, stage = v_tile % RING;
-                    ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * stage, (v_tile / RING) & 1u, stop, budget));
+                    ok = __all_sync(0xffffffffu, mbar_wait(tail + 8 * (t & 1u), tail_phase >> (t & 1u) & 1u, stop, budget));
                     if (ok && local_row >= u.keys - j * CT) {
-                        const uint32_t at = ring_smem + stage * TILE + local_row * 128 + (D == 128 ? half * CT_BOX : half * 64);
+                        const uint32_t at = v_smem + (t % STAGES) * TILE + local_row * 128 + (D == 128 ? half * CT_BOX : half * 64);
 #pragma unroll
                         for (int i = 0; i < D / 16; i++)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + i * 16), "r"(0) : "memory");
                     }
                     fence_async_smem();
+                    tail_phase ^= 1u << (t & 1u);
                 }
                 tmem_st_wait_all();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * g);
-                if (QBUF == 2 && j == 0) release_queries();
+                if (lane == 0) mbar_arrive(go + 16 * g + 8 * (t & 1u));
                 float s0, s1, s2, s3;
                 unpack_f32x2(sum_a, s0, s1);
                 unpack_f32x2(sum_b, s2, s3);
                 sum += (s0 + s1) + (s2 + s3);
             }
             if (!alive) break;
-            tile += 2 * steps;
             /* While P.V runs: the row's sum, through the slots the other way round (each thread writes the one
              * it has read and reads the one it wrote, so nobody's pending read is overwritten) */
             *their_x = sum;
             alive = meet(true);
             if (!alive) break;
             sum += *my_x;
-            q_count++;
             const size_t unit = unit_of_row();
             const uint32_t head0 = u.head0, split = u.split;
             have = cursor.next(args, u);
@@ -603,7 +628,7 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             if (args.splits > 1) {
                 const size_t at = size_t(split) * args.query_rows * args.heads + unit;
                 if (live && !half) *reinterpret_cast<float2 *>(args.partial_ml + at * 2) = make_float2(reference, sum);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / 2; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(tmem_o + c, o);
@@ -615,17 +640,15 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                                 make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
-                if (lane == 0) mbar_arrive(q_free + 8 * (g * QBUF + (q_count - 1) % QBUF));
             } else {
-                /* All scores -inf: zeros; a NaN sum stays NaN. A whole tile goes through the tile's query buffer
-                 * (its scores are complete) to the copy engine, 32 rows x D / 2 dims per warp: 32 KiB stored
-                 * row by row would cost the shared-memory path a cycle per 16 or 32 bytes, and the tensor
-                 * core reads its operands through the same path. */
+                /* All scores -inf: zeros; a NaN sum stays NaN. Rows of a whole tile leave through the warp's
+                 * staging area and the copy engine, 32 rows x 32 dims at a time: stored row by row they cost
+                 * the shared-memory path a cycle per 16 or 32 bytes, and the tensor core reads its operands
+                 * through the same path. */
                 const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
-                const bool whole = rows == (CT >> args.pack_log2) && args.block_stores;
-                const uint32_t buffer = q_smem + (g * QBUF + (q_count - 1) % QBUF) * TILE + (D == 128 ? half * CT_BOX : 0);
-                const uint32_t line = buffer + local_row * 128, turn = local_row & 7;
-#pragma unroll
+                const bool block = GROUPS == 2 && whole && args.block_stores;
+                const uint32_t area = out_smem + (warp - 2) * CT_OUT, line = area + lane * 64, turn = (lane >> 1) & 3;
+#pragma unroll 1
                 for (int c = 0; c < D / 2; c += 32) {
                     uint32_t o[32], packed[16];
                     tmem_ld32(tmem_o + c, o);
@@ -633,12 +656,20 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         packed[i] = pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-                    if (whole) {
+                    if (block) {
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      /* the area's last block */
+                        __syncwarp();
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; i++) {
-                            const uint32_t chunk = (D == 128 ? 0 : half * 4) + c / 8 + i;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((chunk ^ turn) << 4)),
+                        for (uint32_t i = 0; i < 4; i++)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((i ^ turn) << 4)),
                                          "r"(packed[4 * i]), "r"(packed[4 * i + 1]), "r"(packed[4 * i + 2]), "r"(packed[4 * i + 3]) : "memory");
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                                         ::"l"(&map_out), "r"(area), "r"(int(half * (D / 2) + c)), "r"(int(head0)),
+                                           "r"(int(q_row + (quarter * 32 >> args.pack_log2))) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
                     } else if (live) {
 #pragma unroll
@@ -647,25 +678,11 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                                 make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
                     }
                 }
-                if (whole) {
-                    fence_async_smem();
-                    /* 64-dim lines: with head_dim 64 the two warps of a row fill one line together */
-                    if (D == 64) meet(true);
-                    __syncwarp();
-                    if (lane == 0 && (D == 128 || half == 0)) {
-                        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-                                     ::"l"(&map_out), "r"(buffer + quarter * 32 * 128), "r"(D == 128 ? int(half * 64) : 0), "r"(int(head0)),
-                                       "r"(int(q_row + (quarter * 32 >> args.pack_log2))) : "memory");
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    }
-                }
-                pending = true;
-                if (QBUF == 1 || !have) release_queries();
             }
             /* O has been read: the next unit's P.V waits for this group's next P */
             tc_fence_before();
         }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (GROUPS == 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     __syncwarp();
@@ -720,18 +737,19 @@ h3b_cross_merge(const CrossArgs args) {
     for (int i = 0; i < D / 32; i++) args.out[unit * D + lane + 32 * i] = to_bf16(o[i] * inv);
 }
 
-/* [rows][heads][D] BF16 as a 3-D tensor (dim, head, row); box = 64 dims x box_heads x box_rows */
-bool ct_map(CUtensorMap *map, const uint16_t *data, uint32_t rows, uint32_t heads, uint32_t dim, uint32_t box_heads,
-            uint32_t box_rows) {
+/* [rows][heads][D] BF16 as a 3-D tensor (dim, head, row); box = box_dims (64 or 32, one swizzled line) x
+ * box_heads x box_rows */
+bool ct_map(CUtensorMap *map, const uint16_t *data, uint32_t rows, uint32_t heads, uint32_t dim, uint32_t box_dims,
+            uint32_t box_heads, uint32_t box_rows) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return false;
     cuuint64_t dims[3] = {dim, heads, rows};
     cuuint64_t strides[2] = {cuuint64_t(dim) * 2, cuuint64_t(heads) * dim * 2};
-    cuuint32_t box[3] = {64, box_heads, box_rows};
+    cuuint32_t box[3] = {box_dims, box_heads, box_rows};
     cuuint32_t elem[3] = {1, 1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(data), dims, strides, box, elem,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, box_dims == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 /* cudaFuncSetAttribute belongs to a device; one answer per device and kernel */
@@ -757,16 +775,26 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
     CUtensorMap map_q, map_k, map_v, map_out;
     /* a warp's block of the output is 32 tile rows */
     args.block_stores = args.pack <= 32;
-    if (!ct_map(&map_out, args.out, args.query_rows, args.heads, D, args.block_stores ? args.pack : 1,
+    if (!ct_map(&map_out, args.out, args.query_rows, args.heads, D, 32, args.block_stores ? args.pack : 1,
                 args.block_stores ? 32 >> args.pack_log2 : 32) ||
-        !ct_map(&map_q, q, args.query_rows, args.heads, D, args.pack, CT >> args.pack_log2) ||
-        !ct_map(&map_k, k, args.key_rows, args.kv_heads, D, 1, CT) || !ct_map(&map_v, v, args.key_rows, args.kv_heads, D, 1, CT))
+        !ct_map(&map_q, q, args.query_rows, args.heads, D, 64, args.pack, CT >> args.pack_log2) ||
+        !ct_map(&map_k, k, args.key_rows, args.kv_heads, D, 64, 1, CT) ||
+        !ct_map(&map_v, v, args.key_rows, args.kv_heads, D, 64, 1, CT))
         return h3b_fail(gpu, "cannot encode the cross attention tensor maps");
     /* most units there can be: every segment may end in a part of a tile */
     const uint64_t per_item = uint64_t(GROUPS) * CT >> args.pack_log2;
-    const uint64_t units = (args.query_rows / per_item + args.segment_count) * args.head_units * args.splits;
-    if (units > 0xffffffffull - gpu->sm_count * 2) return h3b_fail(gpu, "cross attention has too many tiles");
-    const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2);
+    uint64_t units = (args.query_rows / per_item + args.segment_count) * args.head_units;
+    const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2), tiles = (args.key_rows + CT - 1) / CT;
+    /* The keys of a unit are split where the units alone leave SMs idle. Few rows: up to three units per
+     * resident CTA, which evens out segments of different lengths (four single rows over 512, 77, 2,048
+     * and 1 keys x 56 heads: 40 us unsplit, 34 in two, 30 in four, 31 in eight parts). Many rows: one
+     * round of CTAs, two key tiles or more each, since every part writes its rows in F32. */
+    uint64_t splits = GROUPS == 1 ? (3 * resident + units - 1) / units : resident / units;
+    const uint64_t most = GROUPS == 1 ? tiles : tiles / 2;
+    splits = splits > most ? most : splits;
+    args.splits = splits < 1 ? 1 : uint32_t(splits);
+    units *= args.splits;
+    if (units > 0xffffffffull - 2 * resident) return h3b_fail(gpu, "cross attention has too many tiles");
     const unsigned grid = unsigned(units < resident ? units : resident);
     args.step_h = grid % args.head_units;
     args.step_s = grid / args.head_units % args.splits;
@@ -785,7 +813,7 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
     return h3b_launched(gpu, "cross_sdpa_bf16", H3B_SDPA);
 }
 
-bool env_on(const char *name) {
+bool cross_env_on(const char *name) {
     const char *v = getenv(name);
     return v && *v && strcmp(v, "0") != 0;
 }
@@ -826,7 +854,7 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
     uint16_t *out = h3b_ptr<uint16_t>(output);
 
     const bool aligned = h3b_aligned16(q) && h3b_aligned16(k) && h3b_aligned16(v) && h3b_aligned16(out);
-    if ((head_dim == 64 || head_dim == 128) && aligned && key_rows && scale > 0.0f && !env_on("H3B_SDPA_SIMT")) {
+    if ((head_dim == 64 || head_dim == 128) && aligned && key_rows && scale > 0.0f && !cross_env_on("H3B_SDPA_SIMT")) {
         CrossArgs args = {};
         args.out = out;
         args.segments = table;
@@ -844,8 +872,6 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
         args.units_per_kv = group / args.pack;
         args.scale_log2 = scale * 1.4426950408889634f;
         const bool few = query_rows <= uint64_t(segment_count) * (CT >> args.pack_log2);
-        args.splits = 1;
-        if (const char *force = getenv("H3B_CROSS_SPLITS")) args.splits = uint32_t(atoi(force));
         if (few) return head_dim == 128 ? ct_launch<128, 1>(gpu, args, q, k, v) : ct_launch<64, 1>(gpu, args, q, k, v);
         return head_dim == 128 ? ct_launch<128, 2>(gpu, args, q, k, v) : ct_launch<64, 2>(gpu, args, q, k, v);
     }
