@@ -239,6 +239,7 @@ enum h3b_gemm_epilogue {
     H3B_EPI_SWIGLU = 1,   /* W = [gate rows | up rows]; out[r][c] = swiglu, n = hidden */
     H3B_EPI_QKV_ROPE = 2, /* grouped QKV: per-head RMSNorm + RoPE, writes q/k/v directly   */
     H3B_EPI_STORE_F32 = 3, /* out[r][c] = acc + bias[c], F32 output and bias                */
+    H3B_EPI_LORA = 4,      /* the store with low-rank adapters as further K blocks (h3b_lora.cuh) */
 };
 /* Fused QKV projection + per-head RMSNorm + RoPE for head_dim 128, rope_half 48, grouped
  * layout. Returns -1 when the shape cannot take the fused kernel (caller runs the two-step

@@ -37,9 +37,11 @@
  * pointers, F32 operands) and problems too small to fill the machine.
  */
 #include "h3b_common.cuh"
+#include "h3b_lora.cuh"
 #include "h3b_sm100.cuh"
 
 #include <cstdlib>
+#include <type_traits>
 
 namespace {
 
@@ -190,6 +192,27 @@ __device__ __forceinline__ void qkv_unit_epilogue(const TcArgs &args, uint32_t l
     __syncwarp();
 }
 
+/* Adapter epilogue (H3B_EPI_LORA): the operands of the extra K blocks. A tile has, behind its own K blocks,
+ * `blocks` blocks of 64 rank columns for each of its entries. */
+struct LoraExtra {
+    CUtensorMap map_t, map_up;      /* t as [rows of all entries][rank8], up as [adapter][n][rank8] */
+    h3b_lora_task task;
+    uint32_t blocks;
+};
+struct NoExtra {};
+template <int EPI>
+using Extra = std::conditional_t<EPI == H3B_EPI_LORA, LoraExtra, NoExtra>;
+
+/* entries of a tile of the adapter epilogue; waits for the launch that wrote them */
+__device__ __forceinline__ uint32_t lora_entries(const LoraExtra &extra, uint32_t m_blk) {
+    h3b_wait_for_launch();
+    return extra.task.counts[m_blk] & ~H3B_LORA_MIXED;
+}
+/* the tile, or its K slice that carries the extra blocks */
+__device__ __forceinline__ bool carries_extra(bool split, uint32_t part, uint32_t slices) { return !split || part + 1 == slices; }
+/* K16 instructions of the extra block `b` of an entry */
+__device__ __forceinline__ uint32_t lora_k16(uint32_t rank, uint32_t b) { return (min(rank - b * 64, 64u) + 15) / 16; }
+
 /* What a worker does in a given pass over its work: whole tiles first, then (at most) one
  * K slice of a split tile. */
 struct WorkItem {
@@ -319,7 +342,7 @@ __device__ __noinline__ bool split_tile_merge(const SplitCall args, uint32_t lan
 template <int EPI>
 __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_addr, uint32_t row,
                                               bool row_ok, uint32_t n_blk, uint32_t stage_smem,
-                                              uint32_t lane) {
+                                              uint32_t lane, const Extra<EPI> &extra) {
                 if (EPI == H3B_EPI_QKV_ROPE) {
                     /* the tile's 256 columns are two whole 128-column units of the grouped row */
     #pragma unroll 1
@@ -406,6 +429,11 @@ __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_
                     }
                 } else {
                     uint16_t *dst = args.out + size_t(row) * args.out_cols + n_blk * BN;
+                    bool mixed = false;
+                    if constexpr (EPI == H3B_EPI_LORA) {
+                        h3b_wait_for_launch();
+                        mixed = row_ok && (extra.task.counts[row / extra.task.tile_rows] & H3B_LORA_MIXED);
+                    }
     #pragma unroll 1
                     for (int c = 0; c < BN / 32; c++) {
                         uint32_t r[32];
@@ -432,6 +460,19 @@ __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_
                                 packed[i] = pack_bf16(__uint_as_float(r[2 * i]),
                                                        __uint_as_float(r[2 * i + 1]));
                         }
+                        if constexpr (EPI == H3B_EPI_LORA) {
+                            if (mixed) {
+                                /* not finite: maybe another row's adapter (see h3b_lora_element) */
+    #pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    float lo = __uint_as_float(r[2 * i]), hi = __uint_as_float(r[2 * i + 1]);
+                                    const uint32_t col = col0 + 2 * i;
+                                    if ((h3b_not_finite(lo) || h3b_not_finite(hi)) && col < args.out_cols)
+                                        packed[i] = pack_bf16(h3b_lora_element(extra.task, row, col),
+                                                              h3b_lora_element(extra.task, row, col + 1));
+                                }
+                            }
+                        }
                         if (row_ok) {
     #pragma unroll
                             for (int v = 0; v < 4; v++)
@@ -444,10 +485,23 @@ __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_
                 }
 }
 
+/* a box of an adapter's up matrix (z = adapter) */
+__device__ __forceinline__ void tma_load_3d_up(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_up_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar_cluster_addr, int x,
+                                                    int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 template <int EPI>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-            TcArgs args) {
+            TcArgs args, const __grid_constant__ Extra<EPI> extra) {
     extern __shared__ uint8_t raw_smem[];
     __shared__ int stop_flag;
     const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
@@ -522,6 +576,20 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
+                if constexpr (EPI == H3B_EPI_LORA) {
+                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
+                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                        if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1, stop, args.wait_cycles)) { alive = false; break; }
+                        const uint32_t e = m_blk * extra.task.max_entries + i / extra.blocks, x = i % extra.blocks * BK;
+                        const uint32_t bar = full_bar + 8 * stage;
+                        const int adapter = int(extra.task.entries[e]);
+                        mbar_expect_tx(bar, A_BYTES + B_BYTES);
+                        tma_load_2d(a_smem + stage * A_BYTES, &extra.map_t, bar, int(x), int(e * BM));
+                        tma_load_3d_up(b_smem + stage * B_BYTES, &extra.map_up, bar, int(x), int(n_blk * BN), adapter);
+                        tma_load_3d_up(b_smem + stage * B_BYTES + B_BYTES / 2, &extra.map_up, bar, int(x), int(n_blk * BN + 128), adapter);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                    }
+                }
             }
         }
     } else if (warp == 1) {
@@ -554,6 +622,23 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     umma_commit_if(empty_bar + 8 * stage, leader);
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
+                if constexpr (EPI == H3B_EPI_LORA) {
+                    uint32_t m_blk, n_blk;
+                    tile_coords(item.tile, m_blk, n_blk);
+                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
+                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + 8 * stage, phase, stop, args.wait_cycles))) {
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a_lo = a_lo0 + stage * (A_BYTES >> 4), b_lo = b_lo0 + stage * (B_BYTES >> 4);
+                        const uint32_t k16 = lora_k16(extra.task.rank, i % extra.blocks);
+                        for (uint32_t k = 0; k < k16; k++) umma_ss<true>(d_tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
+                        umma_commit_if(empty_bar + 8 * stage, leader);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                    }
+                }
                 if (!alive) break;
                 umma_commit_if(acc_full + 8 * acc, leader);
                 if (++acc == 2) { acc = 0; acc_phase ^= 1; }
@@ -577,7 +662,7 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                            args.split_tiles, args.split, item.slot, item.part},
                                  lane_addr, quarter * 32 + lane, BM, 4, lane, stop))
                 tile_epilogue<EPI>(args, lane_addr, row, row_ok, n_blk,
-                                   bars + 256 + quarter * QKV_STAGE_BYTES, lane);
+                                   bars + 256 + quarter * QKV_STAGE_BYTES, lane, extra);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
@@ -625,7 +710,7 @@ constexpr size_t pair_smem() {
 template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
 h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              TcArgs args) {
+              TcArgs args, const __grid_constant__ Extra<EPI> extra) {
     constexpr int NS = pair_stages<EPI>();
     extern __shared__ uint8_t raw_smem[];
     __shared__ int stop_flag;
@@ -697,6 +782,19 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     tma_load_2d_pair(b_smem + stage * (B_BYTES / 2), &map_b, bar, int(kb * BK), b_row);
                     if (++stage == NS) { stage = 0; phase ^= 1; }
                 }
+                if constexpr (EPI == H3B_EPI_LORA) {
+                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
+                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                        if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1, stop, args.wait_cycles)) { alive = false; break; }
+                        const uint32_t e = m_blk * extra.task.max_entries + i / extra.blocks, x = i % extra.blocks * BK;
+                        const uint32_t bar = cluster_map(full_bar + 8 * stage, 0);
+                        const int adapter = int(extra.task.entries[e]);
+                        if (rank == 0) mbar_expect_tx(full_bar + 8 * stage, 2 * PAIR_STAGE_BYTES);
+                        tma_load_2d_pair(a_smem + stage * A_BYTES, &extra.map_t, bar, int(x), int(e * 2 * BM + rank * BM));
+                        tma_load_3d_up_pair(b_smem + stage * (B_BYTES / 2), &extra.map_up, bar, int(x), int(n_blk * BN + rank * 128), adapter);
+                        if (++stage == NS) { stage = 0; phase ^= 1; }
+                    }
+                }
             }
         }
     } else if (warp == 1) {
@@ -728,6 +826,23 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     umma_commit_pair_if(empty_bar + 8 * stage, leader);
                     if (++stage == NS) { stage = 0; phase ^= 1; }
                 }
+                if constexpr (EPI == H3B_EPI_LORA) {
+                    uint32_t m_blk, n_blk;
+                    tile_coords(item.tile, m_blk, n_blk);
+                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
+                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + 8 * stage, phase, stop, args.wait_cycles))) {
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a_lo = a_lo0 + stage * (A_BYTES >> 4), b_lo = b_lo0 + stage * ((B_BYTES / 2) >> 4);
+                        const uint32_t k16 = lora_k16(extra.task.rank, i % extra.blocks);
+                        for (uint32_t k = 0; k < k16; k++) umma_ss_pair<true>(d_tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
+                        umma_commit_pair_if(empty_bar + 8 * stage, leader);
+                        if (++stage == NS) { stage = 0; phase ^= 1; }
+                    }
+                }
                 if (!alive) break;
                 umma_commit_pair_if(acc_full + 8 * acc, leader);
                 if (++acc == 2) { acc = 0; acc_phase ^= 1; }
@@ -750,7 +865,7 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                                            args.split_tiles, args.split, item.slot, item.part},
                                  lane_addr, rank * BM + quarter * 32 + lane, 2 * BM, 8, lane, stop))
                 tile_epilogue<EPI>(args, lane_addr, row, row < args.rows, n_blk,
-                                   bars + 256 + quarter * QKV_STAGE_BYTES, lane);
+                                   bars + 256 + quarter * QKV_STAGE_BYTES, lane, extra);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(cluster_map(acc_empty + 8 * acc, 0));
@@ -959,11 +1074,51 @@ bool configure_split(h3_gpu *gpu, TcArgs &args, uint32_t workers, uint32_t tile_
     return true;
 }
 
+/* CTA pairs (256 x 256 tiles) when that does not cost an extra round of tiles (a pair tile
+ * occupies each of its two SMs as long as a lone 128 x 256 tile; with few rows the 256-row
+ * granularity wastes more: 800 rows = 7 lone row blocks but 4 x 256), the device can
+ * co-schedule clusters of two, and X fits in L2: measured inside the power-capped step, pairs
+ * win at 6,400 rows (258 vs 265 ms per 50-block step), make no difference at 12,619 rows and
+ * lose at 50,476 rows (1,070 vs 1,024 ms per 10 blocks), where X streams from HBM as well. */
+template <int EPI>
+bool takes_pairs(h3_gpu *gpu, uint32_t rows, uint32_t tiles_n) {
+    const int pairs = max_resident_pairs<EPI>(gpu->device);
+    if (pairs <= 0) return false;
+    bool pair_size = false;
+    if (rows > BM) {
+        const uint64_t lone_rounds = (uint64_t((rows + BM - 1) / BM) * tiles_n + gpu->sm_count - 1) / gpu->sm_count;
+        const uint64_t pair_rounds = (uint64_t((rows + 2 * BM - 1) / (2 * BM)) * tiles_n + pairs - 1) / pairs;
+        pair_size = (rows <= 8192 && pair_rounds <= lone_rounds) || env_flag("H3B_CTA_PAIRS_ALWAYS");
+    }
+    return pair_size && !env_flag("H3B_NO_CTA_PAIRS");
+}
+
+/* launches of the adapter epilogue may begin while the kernel in front of them runs */
+template <int EPI, class Kernel>
+void launch_kernel(h3_gpu *gpu, Kernel *kernel, uint32_t grid, size_t smem, const CUtensorMap &map_a, const CUtensorMap &map_b,
+                   const TcArgs &args, const Extra<EPI> &extra) {
+    if constexpr (EPI == H3B_EPI_LORA) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(grid);
+        config.blockDim = dim3(TC_THREADS);
+        config.dynamicSmemBytes = smem;
+        config.stream = gpu->stream;
+        cudaLaunchAttribute attribute;
+        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute.val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        cudaLaunchKernelEx(&config, kernel, map_a, map_b, args, extra);      /* an error is reported by h3b_launched */
+    } else {
+        kernel<<<grid, TC_THREADS, smem, gpu->stream>>>(map_a, map_b, args, extra);
+    }
+}
+
 template <int EPI>
 int launch_tc(h3_gpu *gpu, uint16_t *out, const uint16_t *x, const uint16_t *w,
               const uint16_t *bias, uint32_t rows, uint32_t k, uint32_t weight_rows,
               uint32_t out_cols, uint32_t tiles_n, uint32_t up_offset,
-              const TcArgs *extra = nullptr) {
+              const TcArgs *extra = nullptr, const Extra<EPI> &more = Extra<EPI>{}, bool may_split = true) {
     static bool configured_on[64];      /* the attribute is per device */
     static std::mutex configure_mutex;
     constexpr size_t smem_bytes = stages_rows<EPI>() ? TC_SMEM_QKV : TC_SMEM;
@@ -1004,20 +1159,11 @@ int launch_tc(h3_gpu *gpu, uint16_t *out, const uint16_t *x, const uint16_t *w,
         const uint32_t groups = (args.tiles_m + gm - 1) / gm;
         args.group_m = (args.tiles_m + groups - 1) / groups;
     }
-    /* CTA pairs (256 x 256 tiles) when that does not cost an extra round of tiles (a pair tile
-     * occupies each of its two SMs as long as a lone 128 x 256 tile; with few rows the 256-row
-     * granularity wastes more: 800 rows = 7 lone row blocks but 4 x 256), the device can
-     * co-schedule clusters of two, and X fits in L2: measured inside the power-capped step, pairs
-     * win at 6,400 rows (258 vs 265 ms per 50-block step), make no difference at 12,619 rows and
-     * lose at 50,476 rows (1,070 vs 1,024 ms per 10 blocks), where X streams from HBM as well. */
     const int pairs = max_resident_pairs<EPI>(gpu->device);
-    bool pair_size = false;
-    if (pairs > 0 && rows > BM) {
-        const uint64_t lone_rounds = (uint64_t(args.tiles_m) * tiles_n + gpu->sm_count - 1) / gpu->sm_count;
-        const uint64_t pair_rounds = (uint64_t((rows + 2 * BM - 1) / (2 * BM)) * tiles_n + pairs - 1) / pairs;
-        pair_size = (rows <= 8192 && pair_rounds <= lone_rounds) || env_flag("H3B_CTA_PAIRS_ALWAYS");
-    }
-    if (pair_size && pairs > 0 && !env_flag("H3B_NO_CTA_PAIRS")) {
+    bool on_pairs;
+    if constexpr (EPI == H3B_EPI_LORA) on_pairs = more.task.tile_rows == 2 * BM;      /* decided with the entries */
+    else on_pairs = takes_pairs<EPI>(gpu, rows, tiles_n);
+    if (on_pairs) {
         args.tiles_m = (rows + 2 * BM - 1) / (2 * BM);
         const double slab = 2.0 * BM * k * 2.0;
         uint32_t gm = uint32_t(40.0e6 / slab);
@@ -1027,18 +1173,44 @@ int launch_tc(h3_gpu *gpu, uint16_t *out, const uint16_t *x, const uint16_t *w,
         args.group_m = (args.tiles_m + groups - 1) / groups;
         const uint32_t tiles = args.tiles_m * args.tiles_n;
         const uint32_t workers = tiles < uint32_t(pairs) ? tiles : uint32_t(pairs);
-        if (!configure_split(gpu, args, workers, 2 * BM)) return 0;
-        h3b_gemm_pair<EPI><<<2 * workers, TC_THREADS, pair_smem<EPI>(), gpu->stream>>>(map_a, map_b, args);
+        if (may_split && !configure_split(gpu, args, workers, 2 * BM)) return 0;
+        launch_kernel<EPI>(gpu, h3b_gemm_pair<EPI>, 2 * workers, pair_smem<EPI>(), map_a, map_b, args, more);
         return 1;
     }
     uint32_t tiles = args.tiles_m * args.tiles_n;
     uint32_t grid = tiles < uint32_t(gpu->sm_count) ? tiles : uint32_t(gpu->sm_count);
-    if (!configure_split(gpu, args, grid, BM)) return 0;
-    h3b_gemm_tc<EPI><<<grid, TC_THREADS, smem_bytes, gpu->stream>>>(map_a, map_b, args);
+    if (may_split && !configure_split(gpu, args, grid, BM)) return 0;
+    launch_kernel<EPI>(gpu, h3b_gemm_tc<EPI>, grid, smem_bytes, map_a, map_b, args, more);
     return 1;
 }
 
 }  // namespace
+
+uint32_t h3b_gemm_lora_tile_rows(h3_gpu *gpu, uint32_t rows, uint32_t n) {
+    return takes_pairs<H3B_EPI_LORA>(gpu, rows, (n + BN - 1) / BN) ? 2 * BM : BM;
+}
+
+int h3b_gemm_lora(h3_gpu *gpu, const h3b_lora_task &task, bool captured) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return 0;
+    LoraExtra extra = {};
+    extra.task = task;
+    extra.blocks = (task.rank + BK - 1) / BK;
+    const uint64_t tiles = (task.rows + task.tile_rows - 1) / task.tile_rows;
+    if (!make_map(&extra.map_t, task.t, tiles * task.max_entries * task.tile_rows, task.rank8, BM)) return 0;
+    cuuint64_t dims[3] = {task.rank8, task.n, task.adapters};
+    cuuint64_t strides[2] = {cuuint64_t(task.rank8) * 2, cuuint64_t(task.n) * task.rank8 * 2};
+    cuuint32_t box[3] = {BK, 128, 1};
+    cuuint32_t elem[3] = {1, 1, 1};
+    if (encode(&extra.map_up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(task.up8), dims, strides, box, elem,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return 0;
+    /* the split tail round's scratch belongs to the context: a captured launch, which may be replayed beside
+     * others, does without it */
+    return launch_tc<H3B_EPI_LORA>(gpu, task.out, task.x, task.w, task.bias, task.rows, task.k, task.n, task.n,
+                                   (task.n + BN - 1) / BN, 0, nullptr, extra, !captured);
+}
 
 bool h3b_tensor_map_available() { return encode_tiled() != nullptr; }
 

@@ -1,13 +1,22 @@
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[r] = bf16( x[r].W^T + bias + scale[a] (x[r].down[a]^T).up[a]^T ),  a = row_adapter[r].
  *
+ * On the tensor cores a call is two launches. h3b_lora_down_tc finds the adapters that occur in every tile of rows
+ * (its entries, h3b_lora.cuh) and computes their low-rank rows t; the projection then takes t and up as
+ * further K blocks of the tile's accumulation, so the adapters cost no pass over the output and there is
+ * one rounding. The projection is launched as a programmatic dependent: it streams its own K blocks while
+ * the first kernel finishes and waits for t only behind them. Many rows: the 128- and 256-row tiles of
+ * h3b_gemm.cu. Few rows: h3b_lora_rows, which streams the weight through the M side of the instruction.
+ *
  * Kernels that take any shape and alignment (one F32 fmaf chain per sum): h3b_lora_down_simt computes
  * the low-rank row t[r] = scale[a] x[r].down[a]^T once, h3b_lora_simt the projection with t[r].up[a]^T
  * added to every output before its one rounding.
  */
 #include "h3b_common.cuh"
+#include "h3b_lora.cuh"
+#include "h3b_sm100.cuh"
 
-#include <cuda_bf16.h>
+#include <cstdlib>
 
 namespace {
 
@@ -84,7 +93,491 @@ h3b_lora_simt(const uint16_t *x, const uint16_t *w, const uint16_t *bias, const 
     }
 }
 
+/* ------------------------------------------------------------- tensor cores */
+
+constexpr int LR_M = 128;                    /* rows of an instruction: x rows (down) or weight rows (projection) */
+constexpr int LR_K = 64;                     /* one 128-byte swizzle line */
+constexpr int LR_A_BYTES = LR_M * LR_K * 2;
+constexpr int LR_THREADS = 192;              /* TMA, MMA, 4 epilogue warps */
+constexpr int LR_STAGES = 8;                 /* barriers laid out; a launch uses `stages` of them */
+constexpr int LR_BAR_BYTES = 256;
 constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1024;
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+struct RingArgs {
+    int *status;
+    long long wait_cycles;
+    uint32_t stages, stage_bytes, tmem_columns;
+};
+
+/* barriers, the pipeline's shared memory and the accumulator of a CTA of the two kernels below */
+struct Ring {
+    uint32_t stage0, full, empty, done, tmem;
+    volatile int *stop;
+};
+__device__ __forceinline__ Ring ring_setup(const RingArgs &args, uint8_t *raw, int *stop_flag) {
+    Ring r;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    r.stage0 = base;
+    r.full = base + args.stages * args.stage_bytes;
+    r.empty = r.full + 8 * LR_STAGES;
+    r.done = r.empty + 8 * LR_STAGES;
+    r.stop = stop_flag;
+    const uint32_t holder = r.done + 8;
+    if (threadIdx.x == 0) {
+        *stop_flag = 0;
+        for (uint32_t i = 0; i < args.stages; i++) {
+            mbar_init(r.full + 8 * i, 1);
+            mbar_init(r.empty + 8 * i, 1);
+        }
+        mbar_init(r.done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x >> 5 == 1) tmem_alloc(holder, args.tmem_columns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r.tmem) : "r"(holder));
+    return r;
+}
+__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r) {
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*r.stop) {
+        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_GEMM_TIMEOUT));
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (threadIdx.x >> 5 == 1) {
+        tc_fence_after();
+        tmem_free(r.tmem, args.tmem_columns);
+    }
+}
+
+/* t of one 128-row block for up to `group` entries of its tile: x block . [down of the entries]^T, K split over
+ * the CTAs of a cluster, partial sums joined through distributed shared memory in rank order. Every row
+ * then takes its own adapter's columns. Bound by reading x once (6,400 x 5,376: 69 MB, 10.5 us). */
+struct DownArgs {
+    h3b_lora_task task;
+    RingArgs ring;
+    uint32_t k_blocks, rank16, group;        /* columns per entry (rank rounded up to 16); entries per cluster */
+};
+__global__ void __launch_bounds__(LR_THREADS)
+h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_down,
+                 const __grid_constant__ DownArgs args) {
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ int stop_flag;
+    __shared__ uint32_t present[kMaxAdapters / 32], before[kMaxAdapters / 32];
+    __shared__ uint16_t entry[256];
+    __shared__ uint32_t without;
+    const h3b_lora_task &task = args.task;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t split = gridDim.x, part = blockIdx.x, row0 = blockIdx.y * LR_M, tile = row0 / task.tile_rows;
+    h3b_let_next_launch();
+
+    /* the tile's entries: adapters that occur among its rows, ascending */
+    if (threadIdx.x < kMaxAdapters / 32) present[threadIdx.x] = 0;
+    if (threadIdx.x == 0) without = 0;
+    __syncthreads();
+    for (uint32_t r = threadIdx.x; r < task.tile_rows; r += LR_THREADS) {
+        const uint32_t row = tile * task.tile_rows + r;
+        if (row >= task.rows) break;
+        const uint32_t a = task.row_adapter ? task.row_adapter[row] : 0;
+        if (a < task.adapters) atomicOr(&present[a >> 5], 1u << (a & 31));
+        else without = 1;
+    }
+    __syncthreads();
+    uint32_t count = 0;
+    if (warp == 0) {
+        uint32_t mine = present[lane], sum = __popc(mine);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        uint32_t at = sum - __popc(mine);
+        before[lane] = at;
+        for (; mine; mine &= mine - 1) entry[at++] = uint16_t(lane * 32 + __ffs(mine) - 1);
+    }
+    __syncthreads();
+    count = before[31] + __popc(present[31]);
+    const uint32_t e0 = blockIdx.z * args.group, e1 = min(count, e0 + args.group);
+    if (blockIdx.z == 0 && part == 0 && row0 == tile * task.tile_rows) {
+        for (uint32_t e = threadIdx.x; e < count; e += LR_THREADS) task.entries[size_t(tile) * task.max_entries + e] = entry[e];
+        if (threadIdx.x == 0) task.counts[tile] = count | (count > 1 || (count && without) ? H3B_LORA_MIXED : 0u);
+    }
+    if (e0 >= e1) return;                                /* the whole cluster */
+    Ring ring = ring_setup(args.ring, raw_smem, &stop_flag);
+    const uint32_t columns = (e1 - e0) * args.rank16;
+    const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            for (uint32_t kb = kb0; kb < kb1; kb++) {
+                if (!mbar_wait(ring.empty + 8 * stage, phase ^ 1, ring.stop, args.ring.wait_cycles)) break;
+                const uint32_t bar = ring.full + 8 * stage, dst = ring.stage0 + stage * args.ring.stage_bytes;
+                mbar_expect_tx(bar, LR_A_BYTES + columns * LR_K * 2);
+                tma_load_2d(dst, &map_x, bar, int(kb * LR_K), int(row0));
+                for (uint32_t e = e0; e < e1; e++)
+                    tma_load_2d(dst + LR_A_BYTES + (e - e0) * args.rank16 * LR_K * 2, &map_down, bar, int(kb * LR_K), int(entry[e] * task.rank));
+                if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t leader = lane == 0, idesc = instruction_desc(LR_M, int(columns));
+        uint32_t stage = 0, phase = 0;
+        bool alive = true;
+        for (uint32_t kb = kb0; kb < kb1; kb++) {
+            alive = __all_sync(0xffffffffu, mbar_wait(ring.full + 8 * stage, phase, ring.stop, args.ring.wait_cycles));
+            if (!alive) break;
+            tc_fence_after();
+            const uint32_t a_lo = desc_lo_kmajor(ring.stage0 + stage * args.ring.stage_bytes);
+            const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4);
+            if (kb == kb0) umma_ss<false>(ring.tmem, a_lo, b_lo, idesc, leader);
+            else umma_ss<true>(ring.tmem, a_lo, b_lo, idesc, leader);
+#pragma unroll
+            for (int k = 1; k < LR_K / 16; k++) umma_ss<true>(ring.tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
+            umma_commit_if(ring.empty + 8 * stage, leader);
+            if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
+        }
+        if (alive) umma_commit_if(ring.done, leader);
+    } else {
+        /* accumulator -> this CTA's shared memory, [row][columns] F32 with 16-byte pieces XOR-swizzled by row
+         * (every copy and product of this CTA is complete, the stages are free) */
+        const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
+        if (__all_sync(0xffffffffu, mbar_wait(ring.done, 0, ring.stop, args.ring.wait_cycles))) {
+            tc_fence_after();
+            for (uint32_t c = 0; c < columns; c += 16) {
+                uint32_t v[16];
+                asm volatile(
+                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                    : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                      "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                    : "r"(ring.tmem + ((quarter * 32) << 16) + c) : "memory");
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    const uint32_t piece = (c / 4 + i) ^ (row & 3);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ring.stage0 + (row * columns + piece * 4) * 4),
+                                 "r"(v[4 * i]), "r"(v[4 * i + 1]), "r"(v[4 * i + 2]), "r"(v[4 * i + 3]) : "memory");
+                }
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (!*ring.stop) {
+        /* rows part, part + split, ...: the row's own columns of all CTAs, scaled and rounded; zeros for the
+         * entries that are not its own */
+        for (uint32_t r = part + split * warp; r < LR_M && row0 + r < task.rows; r += split * (LR_THREADS / 32)) {
+            const uint32_t a = task.row_adapter ? task.row_adapter[row0 + r] : 0;
+            const uint32_t own = a < task.adapters ? before[a >> 5] + __popc(present[a >> 5] & ((1u << (a & 31)) - 1)) : 0xffffffffu;
+            const float s = own >= e0 && own < e1 && task.scale ? task.scale[a] : 1.0f;
+            for (uint32_t e = e0; e < e1; e++) {
+                uint16_t *dst = task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + (row0 + r) % task.tile_rows) * task.rank8;
+                for (uint32_t j = 2 * lane; j < task.rank8; j += 64) {
+                    float v[2] = {0.0f, 0.0f};
+                    if (e == own)
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+                            if (j + i < task.rank) {
+                                const uint32_t c = (e - e0) * args.rank16 + j + i;
+                                const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4 + c % 4) * 4;
+                                for (uint32_t p = 0; p < split; p++) v[i] += ld_cluster_f32(cluster_map(at, p));
+                                v[i] *= s;
+                            }
+                    *reinterpret_cast<uint32_t *>(dst + j) = pack_bf16(v[0], v[1]);
+                }
+            }
+        }
+    }
+    cluster_sync_all();      /* nobody leaves while its shared memory may be read */
+    ring_close(args.ring, ring);
+}
+
+/* The projection of few rows: D[weight row][x row] = W.x^T for 128 weight rows and a tile of up to 128 x rows, the
+ * weight streamed once through the M side of the instruction. K is split over the CTAs of a cluster so
+ * that every SM pulls on the weight (42 weight tiles of n = 5,376 would leave 106 SMs idle); the last CTA
+ * takes the entries' blocks too. Partial sums are joined through distributed shared memory in rank order.
+ * Bound by the weight's bytes. */
+struct RowsArgs {
+    h3b_lora_task task;
+    RingArgs ring;
+    uint32_t k_blocks, blocks;               /* blocks: K blocks of an entry */
+};
+__global__ void __launch_bounds__(LR_THREADS)
+h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+              const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_t,
+              const __grid_constant__ RowsArgs args) {
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ int stop_flag;
+    const h3b_lora_task &task = args.task;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t split = gridDim.x, part = blockIdx.x, w0 = blockIdx.y * LR_M, tile = blockIdx.z;
+    const uint32_t row0 = tile * task.tile_rows, live = min(task.tile_rows, task.rows - row0);
+    const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
+    const uint32_t b_bytes = task.tile_rows * LR_K * 2;
+    Ring ring = ring_setup(args.ring, raw_smem, &stop_flag);
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool alive = true;
+            auto next_stage = [&]() -> uint32_t {
+                alive = mbar_wait(ring.empty + 8 * stage, phase ^ 1, ring.stop, args.ring.wait_cycles);
+                if (alive) mbar_expect_tx(ring.full + 8 * stage, LR_A_BYTES + b_bytes);
+                return ring.stage0 + stage * args.ring.stage_bytes;
+            };
+            auto advance = [&] { if (++stage == args.ring.stages) { stage = 0; phase ^= 1; } };
+            for (uint32_t kb = kb0; alive && kb < kb1; kb++) {
+                const uint32_t dst = next_stage(), bar = ring.full + 8 * stage;
+                if (!alive) break;
+                tma_load_2d(dst, &map_w, bar, int(kb * LR_K), int(w0));
+                tma_load_2d(dst + LR_A_BYTES, &map_x, bar, int(kb * LR_K), int(row0));
+                advance();
+            }
+            h3b_wait_for_launch();
+            const uint32_t entries = part + 1 == split ? task.counts[tile] & ~H3B_LORA_MIXED : 0;
+            for (uint32_t i = 0; alive && i < entries * args.blocks; i++) {
+                const uint32_t dst = next_stage(), bar = ring.full + 8 * stage, e = tile * task.max_entries + i / args.blocks;
+                if (!alive) break;
+                tma_load_3d(dst, &map_up, bar, int(i % args.blocks * LR_K), int(w0), int(task.entries[e]));
+                tma_load_2d(dst + LR_A_BYTES, &map_t, bar, int(i % args.blocks * LR_K), int(e * task.tile_rows));
+                advance();
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t leader = lane == 0, idesc = instruction_desc(LR_M, int(task.tile_rows));
+        uint32_t stage = 0, phase = 0;
+        bool alive = true, first = true;
+        auto block = [&](uint32_t k16) {
+            alive = __all_sync(0xffffffffu, mbar_wait(ring.full + 8 * stage, phase, ring.stop, args.ring.wait_cycles));
+            if (!alive) return;
+            tc_fence_after();
+            const uint32_t a_lo = desc_lo_kmajor(ring.stage0 + stage * args.ring.stage_bytes);
+            const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4);
+            for (uint32_t k = 0; k < k16; k++) {
+                if (first) umma_ss<false>(ring.tmem, a_lo, b_lo, idesc, leader);
+                else umma_ss<true>(ring.tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
+                first = false;
+            }
+            umma_commit_if(ring.empty + 8 * stage, leader);
+            if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
+        };
+        for (uint32_t kb = kb0; alive && kb < kb1; kb++) block(LR_K / 16);
+        if (part + 1 == split) {
+            h3b_wait_for_launch();
+            const uint32_t entries = task.counts[tile] & ~H3B_LORA_MIXED;
+            for (uint32_t i = 0; alive && i < entries * args.blocks; i++)
+                block((min(task.rank - i % args.blocks * LR_K, uint32_t(LR_K)) + 15) / 16);
+        }
+        if (alive) umma_commit_if(ring.done, leader);
+    } else {
+        /* accumulator -> shared memory [x row][128 weight rows] F32 */
+        const uint32_t quarter = warp & 3;
+        if (__all_sync(0xffffffffu, mbar_wait(ring.done, 0, ring.stop, args.ring.wait_cycles))) {
+            tc_fence_after();
+            for (uint32_t c = 0; c < live; c += 16) {
+                uint32_t v[16];
+                asm volatile(
+                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                    : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                      "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                    : "r"(ring.tmem + ((quarter * 32) << 16) + c) : "memory");
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i++)
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring.stage0 + ((c + i) * LR_M + quarter * 32 + lane) * 4), "r"(v[i]) : "memory");
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (!*ring.stop && threadIdx.x < LR_M) {
+        /* rows part, part + split, ...; a thread has two weight rows of every second of them */
+        h3b_wait_for_launch();
+        const bool mixed = task.counts[tile] & H3B_LORA_MIXED;
+        const uint32_t col = w0 + 2 * (threadIdx.x & 63);
+        if (col < task.n) {
+            float b0 = 0.0f, b1 = 0.0f;
+            if (task.bias) {
+                const uint32_t b = *reinterpret_cast<const uint32_t *>(task.bias + col);
+                b0 = h3b_lo(b);
+                b1 = h3b_hi(b);
+            }
+            for (uint32_t r = part + split * (threadIdx.x >> 6); r < live; r += 2 * split) {
+                const uint32_t at = ring.stage0 + (r * LR_M + 2 * (threadIdx.x & 63)) * 4;
+                float v0 = 0.0f, v1 = 0.0f;
+                for (uint32_t p = 0; p < split; p++) {
+                    const uint32_t from = cluster_map(at, p);
+                    float x0, x1;
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x0), "=f"(x1) : "r"(from) : "memory");
+                    v0 += x0;
+                    v1 += x1;
+                }
+                v0 += b0;
+                v1 += b1;
+                if (mixed && (h3b_not_finite(v0) || h3b_not_finite(v1))) {
+                    v0 = h3b_lora_element(task, row0 + r, col);
+                    v1 = h3b_lora_element(task, row0 + r, col + 1);
+                }
+                *reinterpret_cast<uint32_t *>(task.out + size_t(row0 + r) * task.n + col) = pack_bf16(v0, v1);
+            }
+        }
+    }
+    cluster_sync_all();
+    ring_close(args.ring, ring);
+}
+
+/* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes */
+__global__ void h3b_lora_pad_up(const uint16_t *up, uint16_t *up8, size_t rows, uint32_t rank, uint32_t rank8) {
+    const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= rows * rank8) return;
+    const size_t row = i / rank8;
+    const uint32_t j = uint32_t(i % rank8);
+    up8[i] = j < rank ? up[row * rank + j] : 0;
+}
+
+/* row-major BF16 [rows][k], box of 64 columns x box_rows, 128-byte swizzle */
+bool lora_map(CUtensorMap *map, const uint16_t *data, uint64_t rows, uint64_t k, uint32_t box_rows) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    cuuint64_t dims[2] = {k, rows};
+    cuuint64_t strides[1] = {k * 2};
+    cuuint32_t box[2] = {LR_K, box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(data), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool lora_env(const char *name) {
+    const char *v = getenv(name);
+    return v && *v && strcmp(v, "0") != 0;
+}
+
+/* shared memory of a launch of the two kernels above: `stages` stages, at least what the joined accumulators
+ * need, and the barriers */
+size_t ring_smem(const RingArgs &ring) { return size_t(ring.stages) * ring.stage_bytes + 1024 + LR_BAR_BYTES; }
+
+bool lora_configure(int device) {
+    static std::mutex mutex;
+    static bool done[64];
+    std::lock_guard<std::mutex> guard(mutex);
+    if (!done[device & 63]) {
+        if (cudaFuncSetAttribute(h3b_lora_down_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10) != cudaSuccess ||
+            cudaFuncSetAttribute(h3b_lora_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        done[device & 63] = true;
+    }
+    return true;
+}
+
+template <class Kernel, class... Args>
+void launch_cluster(h3_gpu *gpu, Kernel *kernel, dim3 grid, uint32_t cluster, size_t smem, bool dependent, const Args &...args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(LR_THREADS);
+    config.dynamicSmemBytes = smem;
+    config.stream = gpu->stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = cluster;
+    attributes[0].val.clusterDim.y = 1;
+    attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
+    config.numAttrs = dependent ? 2 : 1;
+    cudaLaunchKernelEx(&config, kernel, args...);      /* an error is reported by h3b_launched */
+}
+
+uint32_t tmem_columns_for(uint32_t columns) {
+    uint32_t n = 32;
+    while (n < columns) n *= 2;
+    return n;
+}
+
+/* CTAs of a cluster that split K: as many as the device can run beside each other, at least 4 K blocks each */
+uint32_t split_for(uint64_t tiles, uint64_t resident, uint32_t k_blocks) {
+    uint64_t split = resident / (tiles ? tiles : 1);
+    if (split > 8) split = 8;
+    if (split > k_blocks / 4) split = k_blocks / 4;
+    return split < 1 ? 1 : uint32_t(split);
+}
+
+/* Rows [0, task.rows) on the tensor cores; scratch as laid out by the caller. */
+int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool captured) {
+    const uint32_t k_blocks = (task.k + LR_K - 1) / LR_K;
+    const uint32_t tiles = (task.rows + task.tile_rows - 1) / task.tile_rows, row_blocks = (task.rows + LR_M - 1) / LR_M;
+    CUtensorMap map_x, map_down;
+    DownArgs down = {};
+    down.task = task;
+    down.k_blocks = k_blocks;
+    down.rank16 = (task.rank + 15) & ~15u;
+    down.group = 256 / down.rank16;
+    if (down.group > task.max_entries) down.group = task.max_entries;
+    const uint32_t groups = (task.max_entries + down.group - 1) / down.group, columns = down.group * down.rank16;
+    down.ring.status = gpu->status_device;
+    down.ring.wait_cycles = gpu->wait_cycles;
+    down.ring.stage_bytes = LR_A_BYTES + columns * LR_K * 2;
+    down.ring.tmem_columns = tmem_columns_for(columns);
+    /* two CTAs per SM where the stages allow it; the joined accumulators (128 x columns F32) have to fit */
+    const uint32_t want = columns <= 64 ? 100 << 10 : 200 << 10;
+    down.ring.stages = want / down.ring.stage_bytes;
+    if (down.ring.stages > uint32_t(LR_STAGES)) down.ring.stages = LR_STAGES;
+    const uint64_t resident = uint64_t(gpu->sm_count) * (columns <= 64 ? 2 : 1);
+    const uint32_t down_split = split_for(row_blocks, resident, k_blocks);
+    if (!lora_map(&map_x, task.x, task.rows, task.k, LR_M) ||
+        !lora_map(&map_down, task.down, uint64_t(task.adapters) * task.rank, task.k, down.rank16))
+        return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
+    launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, groups), down_split, ring_smem(down.ring), false, map_x, map_down, down);
+    if (cudaGetLastError() != cudaSuccess) return h3b_fail(gpu, "linear_lora_bf16: the low-rank rows cannot be launched");
+    if (!few) {
+        if (!h3b_gemm_lora(gpu, task, captured)) return h3b_fail(gpu, "linear_lora_bf16: cannot set up the tensor-core GEMM");
+        return 1;
+    }
+    RowsArgs rows = {};
+    rows.task = task;
+    rows.k_blocks = k_blocks;
+    rows.blocks = (task.rank + LR_K - 1) / LR_K;
+    rows.ring.status = gpu->status_device;
+    rows.ring.wait_cycles = gpu->wait_cycles;
+    rows.ring.stage_bytes = LR_A_BYTES + task.tile_rows * LR_K * 2;
+    rows.ring.tmem_columns = tmem_columns_for(task.tile_rows);
+    rows.ring.stages = (106 << 10) / rows.ring.stage_bytes;
+    if (rows.ring.stages > uint32_t(LR_STAGES)) rows.ring.stages = LR_STAGES;
+    const uint32_t weight_tiles = (task.n + LR_M - 1) / LR_M;
+    const uint32_t split = split_for(uint64_t(weight_tiles) * tiles, uint64_t(gpu->sm_count) * 2, k_blocks);
+    CUtensorMap map_w, map_rows, map_up, map_t;
+    EncodeTiled encode = encode_tiled();
+    cuuint64_t dims[3] = {task.rank8, task.n, task.adapters};
+    cuuint64_t strides[2] = {cuuint64_t(task.rank8) * 2, cuuint64_t(task.n) * task.rank8 * 2};
+    cuuint32_t box[3] = {LR_K, LR_M, 1};
+    cuuint32_t elem[3] = {1, 1, 1};
+    if (!lora_map(&map_w, task.w, task.n, task.k, LR_M) || !lora_map(&map_rows, task.x, task.rows, task.k, task.tile_rows) ||
+        !lora_map(&map_t, task.t, uint64_t(tiles) * task.max_entries * task.tile_rows, task.rank8, task.tile_rows) ||
+        encode(&map_up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(task.up8), dims, strides, box, elem,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
+    launch_cluster(gpu, h3b_lora_rows, dim3(split, weight_tiles, tiles), split, ring_smem(rows.ring), true, map_w, map_rows, map_up, map_t, rows);
+    return 1;
+}
 
 }  // namespace
 
@@ -119,6 +612,55 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
     const uint32_t *map = row_adapter ? h3b_ptr<uint32_t>(row_adapter) : nullptr;
     uint16_t *y = h3b_ptr<uint16_t>(output);
 
+    const bool aligned = h3b_aligned16(x) && h3b_aligned16(w) && (!b || h3b_aligned16(b)) && h3b_aligned16(d) && h3b_aligned16(u) && h3b_aligned16(y);
+    if (aligned && input_dim && input_dim % 8 == 0 && output_dim % 8 == 0 && !lora_env("H3B_NO_TENSOR_CORES") &&
+        double(rows) * output_dim * input_dim >= 32.0 * 256 * 256) {      /* tiny problems are latency bound either way */
+        if (!lora_configure(gpu->device)) return h3b_fail(gpu, "cannot reserve shared memory for the adapter kernels");
+        h3b_lora_task task = {};
+        task.x = x; task.w = w; task.bias = b; task.down = d; task.up = task.up8 = u;
+        task.scale = s;
+        task.row_adapter = map;
+        task.out = y;
+        task.rows = rows; task.k = input_dim; task.n = output_dim; task.adapters = adapters; task.rank = rank;
+        task.rank8 = (rank + 7) & ~7u;
+        /* the weight-streaming kernel while the tiles of the GEMM would leave SMs idle */
+        bool few = uint64_t((rows + 127) / 128) * ((output_dim + 255) / 256) < uint64_t(gpu->sm_count);
+        if (const char *force = getenv("H3B_LORA_FEW")) few = atoi(force);
+        const uint32_t tile_rows = few ? (rows >= 128 ? 128 : (rows + 15) & ~15u) : h3b_gemm_lora_tile_rows(gpu, rows, output_dim);
+        task.tile_rows = tile_rows;
+        task.max_entries = adapters < tile_rows ? adapters : tile_rows;
+        auto rounded = [](size_t bytes) { return (bytes + 255) & ~size_t(255); };
+        /* room for every adapter in every tile; so many rows at a time that it stays within a gigabyte */
+        const size_t tile_bytes = size_t(task.max_entries) * tile_rows * task.rank8 * 2;
+        size_t chunk_tiles = (size_t(1) << 30) / tile_bytes;
+        const size_t all_tiles = (rows + tile_rows - 1) / tile_rows;
+        if (chunk_tiles > all_tiles) chunk_tiles = all_tiles;
+        const size_t t_bytes = rounded(chunk_tiles * tile_bytes);
+        const size_t up_bytes = task.rank8 == rank ? 0 : rounded(size_t(adapters) * output_dim * task.rank8 * 2);
+        const size_t count_bytes = rounded(chunk_tiles * 4), entry_bytes = rounded(chunk_tiles * task.max_entries * 4);
+        h3b_scratch scratch(gpu, t_bytes + up_bytes + count_bytes + entry_bytes);
+        if (!scratch.data) return h3b_fail(gpu, "linear_lora_bf16: cannot allocate the low-rank rows");
+        uint8_t *at = static_cast<uint8_t *>(scratch.data);
+        task.t = reinterpret_cast<uint16_t *>(at);
+        task.counts = reinterpret_cast<uint32_t *>(at + t_bytes + up_bytes);
+        task.entries = reinterpret_cast<uint32_t *>(at + t_bytes + up_bytes + count_bytes);
+        if (up_bytes) {
+            uint16_t *up8 = reinterpret_cast<uint16_t *>(at + t_bytes);
+            const size_t up_rows = size_t(adapters) * output_dim;
+            h3b_lora_pad_up<<<unsigned((up_rows * task.rank8 + 255) / 256), 256, 0, gpu->stream>>>(u, up8, up_rows, rank, task.rank8);
+            task.up8 = up8;
+        }
+        for (size_t tile = 0; tile < all_tiles; tile += chunk_tiles) {
+            const size_t row0 = tile * tile_rows;
+            h3b_lora_task part = task;
+            part.rows = uint32_t(rows - row0 < chunk_tiles * tile_rows ? rows - row0 : chunk_tiles * tile_rows);
+            part.x = x + row0 * input_dim;
+            part.out = y + row0 * output_dim;
+            part.row_adapter = map ? map + row0 : nullptr;
+            if (!lora_tensor_cores(gpu, part, few, scratch.captured)) return 0;
+        }
+        return h3b_launched(gpu, "linear_lora_bf16", kind);
+    }
     h3b_scratch scratch(gpu, size_t(rows) * rank * sizeof(float));
     if (!scratch.data) return h3b_fail(gpu, "linear_lora_bf16: cannot allocate the low-rank rows");
     float *t = static_cast<float *>(scratch.data);
