@@ -760,7 +760,9 @@ bool ct_configure(int device) {
     std::lock_guard<std::mutex> guard(mutex);
     if (!done[device & 63]) {
         if (cudaFuncSetAttribute(h3b_cross_tc<D, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 int(ct_smem<D, GROUPS>())) != cudaSuccess) {
+                                 int(ct_smem<D, GROUPS>())) != cudaSuccess ||
+            cudaFuncSetAttribute(h3b_cross_tc<D, GROUPS>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
             cudaGetLastError();
             return false;
         }

@@ -203,15 +203,21 @@ struct NoExtra {};
 template <int EPI>
 using Extra = std::conditional_t<EPI == H3B_EPI_LORA, LoraExtra, NoExtra>;
 
-/* entries of a tile of the adapter epilogue; waits for the launch that wrote them */
-__device__ __forceinline__ uint32_t lora_entries(const LoraExtra &extra, uint32_t m_blk) {
-    h3b_wait_for_launch();
-    return extra.task.counts[m_blk] & ~H3B_LORA_MIXED;
+/* What follows an item's own K blocks: the entries of its tile, unless another K slice of the tile (all but the
+ * last) carries them. Looked up in the middle of the item, so that the count and the first adapter have
+ * arrived when they are needed, and the launch that writes them has long ended. */
+struct LoraAhead {
+    uint32_t entries, adapter;
+};
+__device__ __forceinline__ LoraAhead lora_look(const LoraExtra &extra, uint32_t m_blk, bool carried) {
+    LoraAhead ahead = {0, 0};
+    if (carried) {
+        h3b_wait_for_launch();
+        ahead.entries = extra.task.counts[m_blk] & ~H3B_LORA_MIXED;
+        ahead.adapter = extra.task.entries[size_t(m_blk) * extra.task.max_entries];
+    }
+    return ahead;
 }
-/* the tile, or its K slice that carries the extra blocks */
-__device__ __forceinline__ bool carries_extra(bool split, uint32_t part, uint32_t slices) { return !split || part + 1 == slices; }
-/* K16 instructions of the extra block `b` of an entry */
-__device__ __forceinline__ uint32_t lora_k16(uint32_t rank, uint32_t b) { return (min(rank - b * 64, 64u) + 15) / 16; }
 
 /* What a worker does in a given pass over its work: whole tiles first, then (at most) one
  * K slice of a split tile. */
@@ -557,7 +563,10 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             for (uint32_t pass = 0; alive && next_item(args, blockIdx.x, gridDim.x, pass, item); pass++) {
                 uint32_t m_blk, n_blk;
                 tile_coords(item.tile, m_blk, n_blk);
+                LoraAhead ahead = {0, 0};
                 for (uint32_t kb = item.kb0; kb < item.kb1; kb++) {
+                    if constexpr (EPI == H3B_EPI_LORA)
+                        if (kb == (item.kb0 + item.kb1) / 2) ahead = lora_look(extra, m_blk, !item.split || item.part + 1 == args.split);
                     if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1, stop, args.wait_cycles)) { alive = false; break; }
                     uint32_t bar = full_bar + 8 * stage;
                     mbar_expect_tx(bar, A_BYTES + B_BYTES);
@@ -577,16 +586,17 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
                 if constexpr (EPI == H3B_EPI_LORA) {
-                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
-                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                    uint32_t x = 0, e = m_blk * extra.task.max_entries, adapter = ahead.adapter, after = 0;
+                    for (uint32_t i = 0; alive && i < ahead.entries * extra.blocks; i++) {
+                        if (x == 0 && i + extra.blocks < ahead.entries * extra.blocks) after = extra.task.entries[e + 1];
                         if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1, stop, args.wait_cycles)) { alive = false; break; }
-                        const uint32_t e = m_blk * extra.task.max_entries + i / extra.blocks, x = i % extra.blocks * BK;
                         const uint32_t bar = full_bar + 8 * stage;
-                        const int adapter = int(extra.task.entries[e]);
                         mbar_expect_tx(bar, A_BYTES + B_BYTES);
                         tma_load_2d(a_smem + stage * A_BYTES, &extra.map_t, bar, int(x), int(e * BM));
-                        tma_load_3d_up(b_smem + stage * B_BYTES, &extra.map_up, bar, int(x), int(n_blk * BN), adapter);
-                        tma_load_3d_up(b_smem + stage * B_BYTES + B_BYTES / 2, &extra.map_up, bar, int(x), int(n_blk * BN + 128), adapter);
+                        tma_load_3d_up(b_smem + stage * B_BYTES, &extra.map_up, bar, int(x), int(n_blk * BN), int(adapter));
+                        tma_load_3d_up(b_smem + stage * B_BYTES + B_BYTES / 2, &extra.map_up, bar, int(x), int(n_blk * BN + 128), int(adapter));
+                        x += BK;
+                        if (x >= extra.blocks * BK) { x = 0; e++; adapter = after; }
                         if (++stage == STAGES) { stage = 0; phase ^= 1; }
                     }
                 }
@@ -605,7 +615,14 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (!__all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, stop, args.wait_cycles))) break;
                 tc_fence_after();
                 uint32_t d_tmem = tmem_base + acc * BN;
+                LoraAhead ahead = {0, 0};
                 for (uint32_t kb = item.kb0; kb < item.kb1; kb++) {
+                    if constexpr (EPI == H3B_EPI_LORA)
+                        if (kb == (item.kb0 + item.kb1) / 2) {
+                            uint32_t m_blk, n_blk;
+                            tile_coords(item.tile, m_blk, n_blk);
+                            ahead = lora_look(extra, m_blk, !item.split || item.part + 1 == args.split);
+                        }
                     if (!__all_sync(0xffffffffu, mbar_wait(full_bar + 8 * stage, phase, stop, args.wait_cycles))) {
                         alive = false;
                         break;
@@ -623,17 +640,16 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
                 if constexpr (EPI == H3B_EPI_LORA) {
-                    uint32_t m_blk, n_blk;
-                    tile_coords(item.tile, m_blk, n_blk);
-                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
-                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                    uint32_t x = 0;
+                    for (uint32_t i = 0; alive && i < ahead.entries * extra.blocks; i++) {
                         if (!__all_sync(0xffffffffu, mbar_wait(full_bar + 8 * stage, phase, stop, args.wait_cycles))) {
                             alive = false;
                             break;
                         }
                         tc_fence_after();
                         const uint32_t a_lo = a_lo0 + stage * (A_BYTES >> 4), b_lo = b_lo0 + stage * (B_BYTES >> 4);
-                        const uint32_t k16 = lora_k16(extra.task.rank, i % extra.blocks);
+                        const uint32_t k16 = (min(extra.task.rank - x, uint32_t(BK)) + 15) / 16;
+                        x = x + BK >= extra.blocks * BK ? 0 : x + BK;
                         for (uint32_t k = 0; k < k16; k++) umma_ss<true>(d_tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
                         umma_commit_if(empty_bar + 8 * stage, leader);
                         if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -774,7 +790,10 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 const int b_row = EPI == H3B_EPI_SWIGLU
                                       ? int((rank ? args.up_offset : 0u) + n_blk * 128)
                                       : int(n_blk * BN + rank * 128);
+                LoraAhead ahead = {0, 0};
                 for (uint32_t kb = item.kb0; kb < item.kb1; kb++) {
+                    if constexpr (EPI == H3B_EPI_LORA)
+                        if (kb == (item.kb0 + item.kb1) / 2) ahead = lora_look(extra, m_blk, !item.split || item.part + 1 == args.split);
                     if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1, stop, args.wait_cycles)) { alive = false; break; }
                     const uint32_t bar = cluster_map(full_bar + 8 * stage, 0);
                     if (rank == 0) mbar_expect_tx(full_bar + 8 * stage, 2 * PAIR_STAGE_BYTES);
@@ -783,15 +802,16 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     if (++stage == NS) { stage = 0; phase ^= 1; }
                 }
                 if constexpr (EPI == H3B_EPI_LORA) {
-                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
-                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                    uint32_t x = 0, e = m_blk * extra.task.max_entries, adapter = ahead.adapter, after = 0;
+                    for (uint32_t i = 0; alive && i < ahead.entries * extra.blocks; i++) {
+                        if (x == 0 && i + extra.blocks < ahead.entries * extra.blocks) after = extra.task.entries[e + 1];
                         if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1, stop, args.wait_cycles)) { alive = false; break; }
-                        const uint32_t e = m_blk * extra.task.max_entries + i / extra.blocks, x = i % extra.blocks * BK;
                         const uint32_t bar = cluster_map(full_bar + 8 * stage, 0);
-                        const int adapter = int(extra.task.entries[e]);
                         if (rank == 0) mbar_expect_tx(full_bar + 8 * stage, 2 * PAIR_STAGE_BYTES);
                         tma_load_2d_pair(a_smem + stage * A_BYTES, &extra.map_t, bar, int(x), int(e * 2 * BM + rank * BM));
-                        tma_load_3d_up_pair(b_smem + stage * (B_BYTES / 2), &extra.map_up, bar, int(x), int(n_blk * BN + rank * 128), adapter);
+                        tma_load_3d_up_pair(b_smem + stage * (B_BYTES / 2), &extra.map_up, bar, int(x), int(n_blk * BN + rank * 128), int(adapter));
+                        x += BK;
+                        if (x >= extra.blocks * BK) { x = 0; e++; adapter = after; }
                         if (++stage == NS) { stage = 0; phase ^= 1; }
                     }
                 }
@@ -810,7 +830,14 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 if (!__all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, stop, args.wait_cycles))) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * BN;
+                LoraAhead ahead = {0, 0};
                 for (uint32_t kb = item.kb0; kb < item.kb1; kb++) {
+                    if constexpr (EPI == H3B_EPI_LORA)
+                        if (kb == (item.kb0 + item.kb1) / 2) {
+                            uint32_t m_blk, n_blk;
+                            tile_coords(item.tile, m_blk, n_blk);
+                            ahead = lora_look(extra, m_blk, !item.split || item.part + 1 == args.split);
+                        }
                     if (!__all_sync(0xffffffffu, mbar_wait(full_bar + 8 * stage, phase, stop, args.wait_cycles))) {
                         alive = false;
                         break;
@@ -827,17 +854,16 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     if (++stage == NS) { stage = 0; phase ^= 1; }
                 }
                 if constexpr (EPI == H3B_EPI_LORA) {
-                    uint32_t m_blk, n_blk;
-                    tile_coords(item.tile, m_blk, n_blk);
-                    const uint32_t entries = alive && carries_extra(item.split, item.part, args.split) ? lora_entries(extra, m_blk) : 0;
-                    for (uint32_t i = 0; alive && i < entries * extra.blocks; i++) {
+                    uint32_t x = 0;
+                    for (uint32_t i = 0; alive && i < ahead.entries * extra.blocks; i++) {
                         if (!__all_sync(0xffffffffu, mbar_wait(full_bar + 8 * stage, phase, stop, args.wait_cycles))) {
                             alive = false;
                             break;
                         }
                         tc_fence_after();
                         const uint32_t a_lo = a_lo0 + stage * (A_BYTES >> 4), b_lo = b_lo0 + stage * ((B_BYTES / 2) >> 4);
-                        const uint32_t k16 = lora_k16(extra.task.rank, i % extra.blocks);
+                        const uint32_t k16 = (min(extra.task.rank - x, uint32_t(BK)) + 15) / 16;
+                        x = x + BK >= extra.blocks * BK ? 0 : x + BK;
                         for (uint32_t k = 0; k < k16; k++) umma_ss_pair<true>(d_tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
                         umma_commit_pair_if(empty_bar + 8 * stage, leader);
                         if (++stage == NS) { stage = 0; phase ^= 1; }

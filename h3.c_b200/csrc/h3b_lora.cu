@@ -103,11 +103,6 @@ constexpr int LR_STAGES = 8;                 /* barriers laid out; a launch uses
 constexpr int LR_BAR_BYTES = 256;
 constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1024;
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -122,35 +117,39 @@ struct RingArgs {
 
 /* barriers, the pipeline's shared memory and the accumulator of a CTA of the two kernels below */
 struct Ring {
-    uint32_t stage0, full, empty, done, tmem;
+    uint32_t stage0, full, empty, done, info, holder;
     volatile int *stop;
 };
-__device__ __forceinline__ Ring ring_setup(const RingArgs &args, uint8_t *raw, int *stop_flag) {
+/* addresses, and (thread 0) the barriers: `arrivals` per full barrier */
+__device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, int *stop_flag, uint32_t arrivals) {
     Ring r;
-    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-    r.stage0 = base;
-    r.full = base + args.stages * args.stage_bytes;
+    r.stage0 = (smem_u32(raw) + 1023u) & ~1023u;
+    r.full = r.stage0 + args.stages * args.stage_bytes;
     r.empty = r.full + 8 * LR_STAGES;
     r.done = r.empty + 8 * LR_STAGES;
+    r.info = r.done + 8;
+    r.holder = r.info + 8;
     r.stop = stop_flag;
-    const uint32_t holder = r.done + 8;
     if (threadIdx.x == 0) {
         *stop_flag = 0;
         for (uint32_t i = 0; i < args.stages; i++) {
-            mbar_init(r.full + 8 * i, 1);
+            mbar_init(r.full + 8 * i, arrivals);
             mbar_init(r.empty + 8 * i, 1);
         }
         mbar_init(r.done, 1);
+        mbar_init(r.info, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (threadIdx.x >> 5 == 1) tmem_alloc(holder, args.tmem_columns);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r.tmem) : "r"(holder));
+    if (threadIdx.x >> 5 == 1) tmem_alloc(r.holder, args.tmem_columns);
     return r;
 }
-__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r) {
+/* behind the block barrier that follows ring_begin: the accumulator's address */
+__device__ __forceinline__ uint32_t ring_tmem(const Ring &r) {
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(r.holder));
+    return tmem;
+}
+__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r, uint32_t tmem) {
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -161,13 +160,59 @@ __device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r) 
     }
     if (threadIdx.x >> 5 == 1) {
         tc_fence_after();
-        tmem_free(r.tmem, args.tmem_columns);
+        tmem_free(tmem, args.tmem_columns);
     }
+}
+
+/* The entries of a tile: the adapters that occur among its rows, ascending. Every CTA finds them for itself. */
+struct Entries {
+    uint32_t present[kMaxAdapters / 32], before[kMaxAdapters / 32];
+    uint16_t adapter[256];          /* of an entry */
+    uint32_t without;
+};
+constexpr uint32_t kNone = 0xffffffffu;
+__device__ __forceinline__ uint32_t adapter_of(const h3b_lora_task &task, uint32_t row) {
+    const uint32_t a = row >= task.rows ? kNone : task.row_adapter ? __ldg(task.row_adapter + row) : 0;
+    return a < task.adapters ? a : kNone;
+}
+/* all threads; returns the number of entries */
+__device__ __forceinline__ uint32_t find_entries(Entries &s, const h3b_lora_task &task, uint32_t tile) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (threadIdx.x < kMaxAdapters / 32) s.present[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.without = 0;
+    __syncthreads();
+    for (uint32_t r = threadIdx.x; r < task.tile_rows && tile * task.tile_rows + r < task.rows; r += blockDim.x) {
+        const uint32_t a = adapter_of(task, tile * task.tile_rows + r);
+        if (a != kNone) atomicOr(&s.present[a >> 5], 1u << (a & 31));
+        else s.without = 1;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        uint32_t mine = s.present[lane], sum = __popc(mine);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= uint32_t(o)) sum += v;
+        }
+        uint32_t at = sum - __popc(mine);
+        s.before[lane] = at;
+        for (; mine; mine &= mine - 1) s.adapter[at++] = uint16_t(lane * 32 + __ffs(mine) - 1);
+    }
+    __syncthreads();
+    return s.before[31] + __popc(s.present[31]);
+}
+__device__ __forceinline__ uint32_t entry_of(const Entries &s, uint32_t a) {
+    return a == kNone ? kNone : s.before[a >> 5] + __popc(s.present[a >> 5] & ((1u << (a & 31)) - 1));
+}
+__device__ __forceinline__ void publish_entries(const Entries &s, const h3b_lora_task &task, uint32_t tile, uint32_t count) {
+    for (uint32_t e = threadIdx.x; e < count; e += blockDim.x) task.entries[size_t(tile) * task.max_entries + e] = s.adapter[e];
+    if (threadIdx.x == 0) task.counts[tile] = count | (count > 1 || (count && s.without) ? H3B_LORA_MIXED : 0u);
 }
 
 /* t of one 128-row block for up to `group` entries of its tile: x block . [down of the entries]^T, K split over
  * the CTAs of a cluster, partial sums joined through distributed shared memory in rank order. Every row
- * then takes its own adapter's columns. Bound by reading x once (6,400 x 5,376: 69 MB, 10.5 us). */
+ * then takes its own adapter's columns. Bound by reading x once (6,400 x 5,376: 69 MB, 10.5 us). The x
+ * copies of the first stages go out before the entries are known. */
 struct DownArgs {
     h3b_lora_task task;
     RingArgs ring;
@@ -178,59 +223,56 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                  const __grid_constant__ DownArgs args) {
     extern __shared__ uint8_t raw_smem[];
     __shared__ int stop_flag;
-    __shared__ uint32_t present[kMaxAdapters / 32], before[kMaxAdapters / 32];
-    __shared__ uint16_t entry[256];
-    __shared__ uint32_t without;
+    __shared__ Entries found;
+    __shared__ uint32_t own[LR_M];           /* entry of a row of the block */
+    __shared__ float own_scale[LR_M];
     const h3b_lora_task &task = args.task;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = gridDim.x, part = blockIdx.x, row0 = blockIdx.y * LR_M, tile = row0 / task.tile_rows;
-    h3b_let_next_launch();
-
-    /* the tile's entries: adapters that occur among its rows, ascending */
-    if (threadIdx.x < kMaxAdapters / 32) present[threadIdx.x] = 0;
-    if (threadIdx.x == 0) without = 0;
-    __syncthreads();
-    for (uint32_t r = threadIdx.x; r < task.tile_rows; r += LR_THREADS) {
-        const uint32_t row = tile * task.tile_rows + r;
-        if (row >= task.rows) break;
-        const uint32_t a = task.row_adapter ? task.row_adapter[row] : 0;
-        if (a < task.adapters) atomicOr(&present[a >> 5], 1u << (a & 31));
-        else without = 1;
-    }
-    __syncthreads();
-    uint32_t count = 0;
-    if (warp == 0) {
-        uint32_t mine = present[lane], sum = __popc(mine);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-        uint32_t at = sum - __popc(mine);
-        before[lane] = at;
-        for (; mine; mine &= mine - 1) entry[at++] = uint16_t(lane * 32 + __ffs(mine) - 1);
-    }
-    __syncthreads();
-    count = before[31] + __popc(present[31]);
-    const uint32_t e0 = blockIdx.z * args.group, e1 = min(count, e0 + args.group);
-    if (blockIdx.z == 0 && part == 0 && row0 == tile * task.tile_rows) {
-        for (uint32_t e = threadIdx.x; e < count; e += LR_THREADS) task.entries[size_t(tile) * task.max_entries + e] = entry[e];
-        if (threadIdx.x == 0) task.counts[tile] = count | (count > 1 || (count && without) ? H3B_LORA_MIXED : 0u);
-    }
-    if (e0 >= e1) return;                                /* the whole cluster */
-    Ring ring = ring_setup(args.ring, raw_smem, &stop_flag);
-    const uint32_t columns = (e1 - e0) * args.rank16;
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
-    if (warp == 0) {
+    h3b_let_next_launch();
+    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 2);
+    const uint32_t early = blockIdx.z == 0 ? min(args.ring.stages, kb1 - kb0) : 0;
+    if (threadIdx.x == 0)
+        for (uint32_t i = 0; i < early; i++) {
+            mbar_expect_tx(ring.full + 8 * i, LR_A_BYTES);
+            tma_load_2d(ring.stage0 + i * args.ring.stage_bytes, &map_x, ring.full + 8 * i, int((kb0 + i) * LR_K), int(row0));
+        }
+    const uint32_t count = find_entries(found, task, tile);
+    const uint32_t e0 = blockIdx.z * args.group, e1 = min(count, e0 + args.group);
+    if (blockIdx.z == 0 && part == 0 && row0 == tile * task.tile_rows) publish_entries(found, task, tile, count);
+    if (threadIdx.x < LR_M) {
+        const uint32_t a = adapter_of(task, row0 + threadIdx.x);
+        own[threadIdx.x] = entry_of(found, a);
+        own_scale[threadIdx.x] = a != kNone && task.scale ? task.scale[a] : 1.0f;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ring_tmem(ring);
+    const bool active = e0 < e1;                         /* the same in the whole cluster */
+    const uint32_t columns = (e1 - e0) * args.rank16;
+    if (!active) {
+        /* nothing to compute; copies that went out have to land before the CTA leaves */
+        if (threadIdx.x == 0)
+            for (uint32_t i = 0; i < early; i++) {
+                mbar_arrive(ring.full + 8 * i);
+                mbar_wait(ring.full + 8 * i, 0, ring.stop, args.ring.wait_cycles);
+            }
+    } else if (warp == 0) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             for (uint32_t kb = kb0; kb < kb1; kb++) {
-                if (!mbar_wait(ring.empty + 8 * stage, phase ^ 1, ring.stop, args.ring.wait_cycles)) break;
                 const uint32_t bar = ring.full + 8 * stage, dst = ring.stage0 + stage * args.ring.stage_bytes;
-                mbar_expect_tx(bar, LR_A_BYTES + columns * LR_K * 2);
-                tma_load_2d(dst, &map_x, bar, int(kb * LR_K), int(row0));
+                if (kb - kb0 >= early) {
+                    if (!mbar_wait(ring.empty + 8 * stage, phase ^ 1, ring.stop, args.ring.wait_cycles)) break;
+                    mbar_expect_tx(bar, LR_A_BYTES);
+                    tma_load_2d(dst, &map_x, bar, int(kb * LR_K), int(row0));
+                }
+                mbar_expect_tx(bar, columns * LR_K * 2);
                 for (uint32_t e = e0; e < e1; e++)
-                    tma_load_2d(dst + LR_A_BYTES + (e - e0) * args.rank16 * LR_K * 2, &map_down, bar, int(kb * LR_K), int(entry[e] * task.rank));
+                    tma_load_2d(dst + LR_A_BYTES + (e - e0) * args.rank16 * LR_K * 2, &map_down, bar, int(kb * LR_K),
+                                int(found.adapter[e] * task.rank));
                 if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
             }
         }
@@ -244,10 +286,10 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             tc_fence_after();
             const uint32_t a_lo = desc_lo_kmajor(ring.stage0 + stage * args.ring.stage_bytes);
             const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4);
-            if (kb == kb0) umma_ss<false>(ring.tmem, a_lo, b_lo, idesc, leader);
-            else umma_ss<true>(ring.tmem, a_lo, b_lo, idesc, leader);
+            if (kb == kb0) umma_ss<false>(tmem, a_lo, b_lo, idesc, leader);
+            else umma_ss<true>(tmem, a_lo, b_lo, idesc, leader);
 #pragma unroll
-            for (int k = 1; k < LR_K / 16; k++) umma_ss<true>(ring.tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
+            for (int k = 1; k < LR_K / 16; k++) umma_ss<true>(tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
             umma_commit_if(ring.empty + 8 * stage, leader);
             if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
         }
@@ -265,7 +307,7 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
                       "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                    : "r"(ring.tmem + ((quarter * 32) << 16) + c) : "memory");
+                    : "r"(tmem + ((quarter * 32) << 16) + c) : "memory");
                 tmem_ld_wait();
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {
@@ -277,34 +319,76 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         }
     }
     __syncwarp();
-    cluster_sync_all();
-    if (!*ring.stop) {
+    if (active) cluster_sync_all();
+    if (active && !*ring.stop) {
         /* rows part, part + split, ...: the row's own columns of all CTAs, scaled and rounded; zeros for the
          * entries that are not its own */
-        for (uint32_t r = part + split * warp; r < LR_M && row0 + r < task.rows; r += split * (LR_THREADS / 32)) {
-            const uint32_t a = task.row_adapter ? task.row_adapter[row0 + r] : 0;
-            const uint32_t own = a < task.adapters ? before[a >> 5] + __popc(present[a >> 5] & ((1u << (a & 31)) - 1)) : 0xffffffffu;
-            const float s = own >= e0 && own < e1 && task.scale ? task.scale[a] : 1.0f;
-            for (uint32_t e = e0; e < e1; e++) {
-                uint16_t *dst = task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + (row0 + r) % task.tile_rows) * task.rank8;
-                for (uint32_t j = 2 * lane; j < task.rank8; j += 64) {
-                    float v[2] = {0.0f, 0.0f};
-                    if (e == own)
-#pragma unroll
-                        for (int i = 0; i < 2; i++)
-                            if (j + i < task.rank) {
-                                const uint32_t c = (e - e0) * args.rank16 + j + i;
-                                const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4 + c % 4) * 4;
-                                for (uint32_t p = 0; p < split; p++) v[i] += ld_cluster_f32(cluster_map(at, p));
-                                v[i] *= s;
-                            }
-                    *reinterpret_cast<uint32_t *>(dst + j) = pack_bf16(v[0], v[1]);
+        const uint32_t mine = (LR_M - part + split - 1) / split, pieces = task.rank8 / 4;
+        const uint32_t items = mine * (e1 - e0) * pieces;
+        for (uint32_t i = threadIdx.x; i < items; i += LR_THREADS) {
+            const uint32_t j = i % pieces * 4, e = e0 + i / pieces % (e1 - e0), r = part + i / pieces / (e1 - e0) * split;
+            if (row0 + r >= task.rows) continue;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (own[r] == e) {
+                const uint32_t c = (e - e0) * args.rank16 + j;
+                const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4) * 4;
+                for (uint32_t p = 0; p < split; p++) {
+                    float4 x;
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_map(at, p)) : "memory");
+                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
                 }
+                const float s = own_scale[r];
+                v.x = j < task.rank ? v.x * s : 0.0f;
+                v.y = j + 1 < task.rank ? v.y * s : 0.0f;
+                v.z = j + 2 < task.rank ? v.z * s : 0.0f;
+                v.w = j + 3 < task.rank ? v.w * s : 0.0f;
             }
+            *reinterpret_cast<uint2 *>(task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + (row0 + r) % task.tile_rows) * task.rank8 + j) =
+                make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
         }
     }
-    cluster_sync_all();      /* nobody leaves while its shared memory may be read */
-    ring_close(args.ring, ring);
+    if (active) cluster_sync_all();      /* nobody leaves while its shared memory may be read */
+    ring_close(args.ring, ring, tmem);
+    h3b_wait_for_launch();               /* the padded up rows, where a launch in front writes them: done before this one is */
+}
+
+/* t of a call of few rows (one tile): a CTA per row and pair of rank indices, four warps to each sum, so that the
+ * kernel costs little more than one memory latency; the tensor-core form above takes 10 us for its set-up,
+ * copies and cluster barriers whatever the size (one row, rank 16, k = 7,168). */
+constexpr int LF_SUMS = 2, LF_WARPS = 4 * LF_SUMS;
+__global__ void __launch_bounds__(32 * LF_WARPS)
+h3b_lora_down_few(const __grid_constant__ h3b_lora_task task) {
+    __shared__ Entries found;
+    __shared__ float part[LF_WARPS];
+    h3b_let_next_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t row = blockIdx.x, j = blockIdx.y * LF_SUMS + warp / 4, a = adapter_of(task, row);
+    float sum = 0.0f;
+    if (a != kNone && j < task.rank) {
+        const uint4 *x = reinterpret_cast<const uint4 *>(task.x + size_t(row) * task.k);
+        const uint4 *d = reinterpret_cast<const uint4 *>(task.down + (size_t(a) * task.rank + j) * task.k);
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (uint32_t i = (warp & 3) * 32 + lane; i < task.k / 8; i += 128) {
+            const uint4 u = __ldg(x + i), v = __ldg(d + i);
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int q = 0; q < 4; q++) s[q] = fmaf(h3b_hi(us[q]), h3b_hi(vs[q]), fmaf(h3b_lo(us[q]), h3b_lo(vs[q]), s[q]));
+        }
+        sum = h3b_warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+    }
+    if (lane == 0) part[warp] = sum;
+    const uint32_t count = find_entries(found, task, 0);          /* has block barriers */
+    if (blockIdx.x == 0 && blockIdx.y == 0) publish_entries(found, task, 0, count);
+    const uint32_t mine = entry_of(found, a);
+    const float s = a != kNone && task.scale ? task.scale[a] : 1.0f;
+    for (uint32_t i = threadIdx.x; i < count * LF_SUMS; i += 32 * LF_WARPS) {
+        const uint32_t e = i / LF_SUMS, q = i % LF_SUMS, jj = blockIdx.y * LF_SUMS + q;
+        const float v = ((part[4 * q] + part[4 * q + 1]) + (part[4 * q + 2] + part[4 * q + 3])) * s;
+        task.t[(size_t(e) * task.tile_rows + row) * task.rank8 + jj] = e == mine && jj < task.rank ? to_bf16(v) : 0;
+    }
+    h3b_wait_for_launch();
 }
 
 /* The projection of few rows: D[weight row][x row] = W.x^T for 128 weight rows and a tile of up to 128 x rows, the
@@ -329,7 +413,17 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const uint32_t row0 = tile * task.tile_rows, live = min(task.tile_rows, task.rows - row0);
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
     const uint32_t b_bytes = task.tile_rows * LR_K * 2;
-    Ring ring = ring_setup(args.ring, raw_smem, &stop_flag);
+    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1);
+    __shared__ uint32_t entries;
+    __shared__ uint16_t adapter[LR_M];
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ring_tmem(ring);
+    /* The entries' blocks are dealt out over the CTAs of the cluster, behind their own: entry e to part e % split.
+     * Which they are is read by a warp that is idle meanwhile: count, adapter and copy in a row would cost the
+     * end of the stream three latencies. */
+    auto extra_blocks = [&] { return (entries + split - 1 - part) / split * args.blocks; };
     if (warp == 0) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
@@ -347,43 +441,51 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 tma_load_2d(dst + LR_A_BYTES, &map_x, bar, int(kb * LR_K), int(row0));
                 advance();
             }
-            h3b_wait_for_launch();
-            const uint32_t entries = part + 1 == split ? task.counts[tile] & ~H3B_LORA_MIXED : 0;
-            for (uint32_t i = 0; alive && i < entries * args.blocks; i++) {
-                const uint32_t dst = next_stage(), bar = ring.full + 8 * stage, e = tile * task.max_entries + i / args.blocks;
+            alive = alive && mbar_wait(ring.info, 0, ring.stop, args.ring.wait_cycles);
+            const uint32_t extra = alive ? extra_blocks() : 0;
+            for (uint32_t i = 0; alive && i < extra; i++) {
+                const uint32_t e = part + i / args.blocks * split, c = i % args.blocks * LR_K;
+                const uint32_t dst = next_stage(), bar = ring.full + 8 * stage;
                 if (!alive) break;
-                tma_load_3d(dst, &map_up, bar, int(i % args.blocks * LR_K), int(w0), int(task.entries[e]));
-                tma_load_2d(dst + LR_A_BYTES, &map_t, bar, int(i % args.blocks * LR_K), int(e * task.tile_rows));
+                tma_load_3d(dst, &map_up, bar, int(c), int(w0), int(adapter[e]));
+                tma_load_2d(dst + LR_A_BYTES, &map_t, bar, int(c), int((tile * task.max_entries + e) * task.tile_rows));
                 advance();
             }
         }
     } else if (warp == 1) {
         const uint32_t leader = lane == 0, idesc = instruction_desc(LR_M, int(task.tile_rows));
-        uint32_t stage = 0, phase = 0;
-        bool alive = true, first = true;
-        auto block = [&](uint32_t k16) {
+        uint32_t stage = 0, phase = 0, blocks = kb1 - kb0;
+        bool alive = true;
+        for (uint32_t i = 0; alive && i <= blocks; i++) {
+            if (i == kb1 - kb0) {      /* how many there are in all is known by now, or soon */
+                alive = __all_sync(0xffffffffu, mbar_wait(ring.info, 0, ring.stop, args.ring.wait_cycles));
+                if (alive) blocks += extra_blocks();
+            }
+            if (!alive || i == blocks) break;
             alive = __all_sync(0xffffffffu, mbar_wait(ring.full + 8 * stage, phase, ring.stop, args.ring.wait_cycles));
-            if (!alive) return;
+            if (!alive) break;
             tc_fence_after();
             const uint32_t a_lo = desc_lo_kmajor(ring.stage0 + stage * args.ring.stage_bytes);
-            const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4);
+            const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4), c = i < kb1 - kb0 ? 0 : (i - (kb1 - kb0)) % args.blocks * LR_K;
+            const uint32_t k16 = i < kb1 - kb0 ? LR_K / 16 : (min(task.rank - c, uint32_t(LR_K)) + 15) / 16;
             for (uint32_t k = 0; k < k16; k++) {
-                if (first) umma_ss<false>(ring.tmem, a_lo, b_lo, idesc, leader);
-                else umma_ss<true>(ring.tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
-                first = false;
+                if (i == 0 && k == 0) umma_ss<false>(tmem, a_lo, b_lo, idesc, leader);
+                else umma_ss<true>(tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
             }
             umma_commit_if(ring.empty + 8 * stage, leader);
             if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
-        };
-        for (uint32_t kb = kb0; alive && kb < kb1; kb++) block(LR_K / 16);
-        if (part + 1 == split) {
-            h3b_wait_for_launch();
-            const uint32_t entries = task.counts[tile] & ~H3B_LORA_MIXED;
-            for (uint32_t i = 0; alive && i < entries * args.blocks; i++)
-                block((min(task.rank - i % args.blocks * LR_K, uint32_t(LR_K)) + 15) / 16);
         }
         if (alive) umma_commit_if(ring.done, leader);
     } else {
+        if (warp == 2) {
+            /* what the launch in front found */
+            h3b_wait_for_launch();
+            const uint32_t count = task.counts[tile] & ~H3B_LORA_MIXED;
+            for (uint32_t e = lane; e < count; e += 32) adapter[e] = uint16_t(task.entries[size_t(tile) * task.max_entries + e]);
+            if (lane == 0) entries = count;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ring.info);
+        }
         /* accumulator -> shared memory [x row][128 weight rows] F32 */
         const uint32_t quarter = warp & 3;
         if (__all_sync(0xffffffffu, mbar_wait(ring.done, 0, ring.stop, args.ring.wait_cycles))) {
@@ -395,7 +497,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
                       "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                    : "r"(ring.tmem + ((quarter * 32) << 16) + c) : "memory");
+                    : "r"(tmem + ((quarter * 32) << 16) + c) : "memory");
                 tmem_ld_wait();
 #pragma unroll
                 for (uint32_t i = 0; i < 16; i++)
@@ -438,16 +540,23 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         }
     }
     cluster_sync_all();
-    ring_close(args.ring, ring);
+    ring_close(args.ring, ring, tmem);
 }
 
-/* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes */
-__global__ void h3b_lora_pad_up(const uint16_t *up, uint16_t *up8, size_t rows, uint32_t rank, uint32_t rank8) {
+/* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes. 8 elements a thread. */
+__global__ void __launch_bounds__(256)
+h3b_lora_pad_up(const uint16_t *__restrict__ up, uint16_t *up8, size_t rows, uint32_t rank, uint32_t rank8) {
+    h3b_let_next_launch();
+    const uint32_t pieces = rank8 / 8;
     const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= rows * rank8) return;
-    const size_t row = i / rank8;
-    const uint32_t j = uint32_t(i % rank8);
-    up8[i] = j < rank ? up[row * rank + j] : 0;
+    if (i >= rows * pieces) return;
+    const size_t row = i / pieces;
+    const uint32_t j = uint32_t(i % pieces) * 8;
+    uint16_t v[8];
+#pragma unroll
+    for (uint32_t q = 0; q < 8; q++) v[q] = j + q < rank ? up[row * rank + j + q] : 0;
+    *reinterpret_cast<uint4 *>(up8 + i * 8) = make_uint4(v[0] | uint32_t(v[1]) << 16, v[2] | uint32_t(v[3]) << 16,
+                                                         v[4] | uint32_t(v[5]) << 16, v[6] | uint32_t(v[7]) << 16);
 }
 
 /* row-major BF16 [rows][k], box of 64 columns x box_rows, 128-byte swizzle */
@@ -478,7 +587,10 @@ bool lora_configure(int device) {
     std::lock_guard<std::mutex> guard(mutex);
     if (!done[device & 63]) {
         if (cudaFuncSetAttribute(h3b_lora_down_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10) != cudaSuccess ||
-            cudaFuncSetAttribute(h3b_lora_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10) != cudaSuccess) {
+            cudaFuncSetAttribute(h3b_lora_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10) != cudaSuccess ||
+            /* two CTAs of 100 KB per SM */
+            cudaFuncSetAttribute(h3b_lora_down_tc, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
+            cudaFuncSetAttribute(h3b_lora_rows, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
             cudaGetLastError();
             return false;
         }
@@ -487,22 +599,30 @@ bool lora_configure(int device) {
     return true;
 }
 
+/* `dependent`: the launch may begin while the kernel in front of it runs, and waits for it inside */
 template <class Kernel, class... Args>
-void launch_cluster(h3_gpu *gpu, Kernel *kernel, dim3 grid, uint32_t cluster, size_t smem, bool dependent, const Args &...args) {
+void launch_cluster(h3_gpu *gpu, Kernel *kernel, dim3 grid, uint32_t threads, uint32_t cluster, size_t smem, bool dependent, const Args &...args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = grid;
-    config.blockDim = dim3(LR_THREADS);
+    config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = gpu->stream;
     cudaLaunchAttribute attributes[2];
-    attributes[0].id = cudaLaunchAttributeClusterDimension;
-    attributes[0].val.clusterDim.x = cluster;
-    attributes[0].val.clusterDim.y = 1;
-    attributes[0].val.clusterDim.z = 1;
-    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    int count = 0;
+    if (cluster > 1) {
+        attributes[count].id = cudaLaunchAttributeClusterDimension;
+        attributes[count].val.clusterDim.x = cluster;
+        attributes[count].val.clusterDim.y = 1;
+        attributes[count].val.clusterDim.z = 1;
+        count++;
+    }
+    if (dependent) {
+        attributes[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[count].val.programmaticStreamSerializationAllowed = 1;
+        count++;
+    }
     config.attrs = attributes;
-    config.numAttrs = dependent ? 2 : 1;
+    config.numAttrs = count;
     cudaLaunchKernelEx(&config, kernel, args...);      /* an error is reported by h3b_launched */
 }
 
@@ -512,12 +632,44 @@ uint32_t tmem_columns_for(uint32_t columns) {
     return n;
 }
 
-/* CTAs of a cluster that split K: as many as the device can run beside each other, at least 4 K blocks each */
-uint32_t split_for(uint64_t tiles, uint64_t resident, uint32_t k_blocks) {
-    uint64_t split = resident / (tiles ? tiles : 1);
-    if (split > 8) split = 8;
-    if (split > k_blocks / 4) split = k_blocks / 4;
-    return split < 1 ? 1 : uint32_t(split);
+/* clusters of `split` CTAs that the device runs beside each other with one CTA per SM; asked once per size. (The
+ * runtime answers for one CTA per SM for kernels that allocate tensor memory, whatever their shared memory;
+ * two of 100 KB do run side by side, checked by their SM numbers and start times.) */
+template <class Kernel>
+uint64_t resident_clusters(int device, Kernel *kernel, uint32_t split, size_t smem) {
+    static std::mutex mutex;
+    static std::unordered_map<uint64_t, int> known;
+    const uint64_t key = uint64_t(device) << 40 | uint64_t(smem) << 8 | split;
+    std::lock_guard<std::mutex> guard(mutex);
+    auto found = known.find(key);
+    if (found != known.end()) return uint64_t(found->second);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(split, 1024);
+    config.blockDim = dim3(LR_THREADS);
+    config.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = split;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+    }
+    return uint64_t(known[key] = clusters);
+}
+
+/* CTAs of a cluster that split K: the most with which all tiles run in one round (a GPC holds whole clusters
+ * only, so clusters of 7 or 8 leave SMs empty), with at least 4 K blocks each. One row, 7,168 -> 5,376, two
+ * CTAs per SM: 21.6 us in 3 parts, 18.5 in 4, 16.8 in 5, 15.9 in 6, 26.3 in 7 (a second round). */
+template <class Kernel>
+uint32_t split_for(h3_gpu *gpu, Kernel *kernel, size_t smem, uint32_t per_sm, uint64_t tiles, uint32_t k_blocks) {
+    for (uint32_t split = 8; split > 1; split--)
+        if (split * 4 <= k_blocks && tiles <= per_sm * resident_clusters(gpu->device, kernel, split, smem)) return split;
+    return 1;
 }
 
 /* Rows [0, task.rows) on the tensor cores; scratch as laid out by the caller. */
@@ -529,23 +681,31 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
     down.task = task;
     down.k_blocks = k_blocks;
     down.rank16 = (task.rank + 15) & ~15u;
-    down.group = 256 / down.rank16;
+    down.group = (down.rank16 <= 128 ? 128 : 256) / down.rank16;
     if (down.group > task.max_entries) down.group = task.max_entries;
     const uint32_t groups = (task.max_entries + down.group - 1) / down.group, columns = down.group * down.rank16;
     down.ring.status = gpu->status_device;
     down.ring.wait_cycles = gpu->wait_cycles;
     down.ring.stage_bytes = LR_A_BYTES + columns * LR_K * 2;
     down.ring.tmem_columns = tmem_columns_for(columns);
-    /* two CTAs per SM where the stages allow it; the joined accumulators (128 x columns F32) have to fit */
-    const uint32_t want = columns <= 64 ? 100 << 10 : 200 << 10;
+    /* two CTAs per SM where there are as many and the joined accumulators (128 x columns F32) leave room for
+     * it; else deeper rings, since a CTA's stream is its bytes in flight over the memory's latency */
+    const bool two = columns <= 128 && uint64_t(row_blocks) * 8 > uint64_t(gpu->sm_count);
+    const uint32_t want = two ? 106 << 10 : 200 << 10;
     down.ring.stages = want / down.ring.stage_bytes;
     if (down.ring.stages > uint32_t(LR_STAGES)) down.ring.stages = LR_STAGES;
-    const uint64_t resident = uint64_t(gpu->sm_count) * (columns <= 64 ? 2 : 1);
-    const uint32_t down_split = split_for(row_blocks, resident, k_blocks);
+    const uint32_t down_split = split_for(gpu, h3b_lora_down_tc, ring_smem(down.ring), two ? 2 : 1, row_blocks, k_blocks);
     if (!lora_map(&map_x, task.x, task.rows, task.k, LR_M) ||
         !lora_map(&map_down, task.down, uint64_t(task.adapters) * task.rank, task.k, down.rank16))
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
-    launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, groups), down_split, ring_smem(down.ring), false, map_x, map_down, down);
+    /* behind the launch that pads up, if there is one */
+    const bool behind = task.up8 != task.up;
+    /* by warps while that reads the inputs a few times at most from L2 */
+    if (few && task.rows <= uint32_t(LR_M) && uint64_t(task.rows) * task.rank <= 2048)
+        launch_cluster(gpu, h3b_lora_down_few, dim3(task.rows, task.rank8 / LF_SUMS), 32 * LF_WARPS, 1, 0, behind, task);
+    else
+        launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, groups), LR_THREADS, down_split, ring_smem(down.ring), behind,
+                       map_x, map_down, down);
     if (cudaGetLastError() != cudaSuccess) return h3b_fail(gpu, "linear_lora_bf16: the low-rank rows cannot be launched");
     if (!few) {
         if (!h3b_gemm_lora(gpu, task, captured)) return h3b_fail(gpu, "linear_lora_bf16: cannot set up the tensor-core GEMM");
@@ -562,7 +722,7 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
     rows.ring.stages = (106 << 10) / rows.ring.stage_bytes;
     if (rows.ring.stages > uint32_t(LR_STAGES)) rows.ring.stages = LR_STAGES;
     const uint32_t weight_tiles = (task.n + LR_M - 1) / LR_M;
-    const uint32_t split = split_for(uint64_t(weight_tiles) * tiles, uint64_t(gpu->sm_count) * 2, k_blocks);
+    const uint32_t split = split_for(gpu, h3b_lora_rows, ring_smem(rows.ring), 2, uint64_t(weight_tiles) * tiles, k_blocks);
     CUtensorMap map_w, map_rows, map_up, map_t;
     EncodeTiled encode = encode_tiled();
     cuuint64_t dims[3] = {task.rank8, task.n, task.adapters};
@@ -575,7 +735,7 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
-    launch_cluster(gpu, h3b_lora_rows, dim3(split, weight_tiles, tiles), split, ring_smem(rows.ring), true, map_w, map_rows, map_up, map_t, rows);
+    launch_cluster(gpu, h3b_lora_rows, dim3(split, weight_tiles, tiles), LR_THREADS, split, ring_smem(rows.ring), true, map_w, map_rows, map_up, map_t, rows);
     return 1;
 }
 
@@ -647,7 +807,7 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
         if (up_bytes) {
             uint16_t *up8 = reinterpret_cast<uint16_t *>(at + t_bytes);
             const size_t up_rows = size_t(adapters) * output_dim;
-            h3b_lora_pad_up<<<unsigned((up_rows * task.rank8 + 255) / 256), 256, 0, gpu->stream>>>(u, up8, up_rows, rank, task.rank8);
+            h3b_lora_pad_up<<<unsigned((up_rows * (task.rank8 / 8) + 255) / 256), 256, 0, gpu->stream>>>(u, up8, up_rows, rank, task.rank8);
             task.up8 = up8;
         }
         for (size_t tile = 0; tile < all_tiles; tile += chunk_tiles) {
