@@ -783,10 +783,11 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
         task.out = y;
         task.rows = rows; task.k = input_dim; task.n = output_dim; task.adapters = adapters; task.rank = rank;
         task.rank8 = (rank + 7) & ~7u;
-        /* the weight-streaming kernel while the tiles of the GEMM would leave SMs idle */
-        bool few = uint64_t((rows + 127) / 128) * ((output_dim + 255) / 256) < uint64_t(gpu->sm_count);
-        if (const char *force = getenv("H3B_LORA_FEW")) few = atoi(force);
-        const uint32_t tile_rows = few ? (rows >= 128 ? 128 : (rows + 15) & ~15u) : h3b_gemm_lora_tile_rows(gpu, rows, output_dim);
+        /* The weight-streaming kernel while one row tile covers the call and the GEMM's tiles would leave SMs idle.
+         * 5,376 -> 5,376, GEMM / streaming: 16 rows 62 / 31 us, 64 54 / 37, 128 54 / 36, 200 42 / 53, 512 40 / 55;
+         * 42 rows 2,688 -> 96,768 (378 GEMM tiles) 105 / 110. */
+        const bool few = rows <= uint32_t(LR_M) && uint64_t((output_dim + 255) / 256) < uint64_t(gpu->sm_count);
+        const uint32_t tile_rows = few ? (rows + 15) & ~15u : h3b_gemm_lora_tile_rows(gpu, rows, output_dim);
         task.tile_rows = tile_rows;
         task.max_entries = adapters < tile_rows ? adapters : tile_rows;
         auto rounded = [](size_t bytes) { return (bytes + 255) & ~size_t(255); };

@@ -71,6 +71,77 @@ class BlockWeights:
             setattr(self, name, tensors[name])
 
 
+class BlockAdapters:
+    """Low-rank adapters of one block's projections, of one or many requests (h3x_linear_lora_bf16; no
+    counterpart in the reference). Each of qkv, out, fc1, fc2 is a pair (down, up) of BF16 tensors,
+    down [adapters][rank][input], up [adapters][output][rank] with the projection's weight rows as
+    outputs, or None for a projection without adapters. row_adapter: U32 [rows], the adapter of every
+    row (0xffffffff: none; a None tensor: adapter 0 for all); scale: F32 [adapters], or None for 1."""
+
+    def __init__(self, *, adapters: int, rank: int, row_adapter: Tensor | None = None, scale: Tensor | None = None,
+                 qkv=None, out=None, fc1=None, fc2=None):
+        self.adapters, self.rank, self.row_adapter, self.scale = adapters, rank, row_adapter, scale
+        self.qkv, self.out, self.fc1, self.fc2 = qkv, out, fc1, fc2
+
+    def project(self, gpu: Gpu, pair, output: Tensor, x: Tensor, weight: Tensor, rows: int, input_dim: int,
+                output_dim: int) -> None:
+        """output = x . weight^T with the adapters of `pair`."""
+        gpu.op("h3x_linear_lora_bf16", output, x, weight, None, pair[0], pair[1], self.scale, self.row_adapter, rows,
+               input_dim, output_dim, self.adapters, self.rank)
+
+
+class Conditioning:
+    """A second attention of the blocks to an encoder's states (h3x_cross_sdpa_bf16; no counterpart in
+    the reference): a block adds softmax(query . states_key^T) states_value to the heads of its joint
+    attention, with the same queries. The states are constant over a denoise run, so their keys and values
+    are projected once (`add_block`); a strength is folded into the value weights.
+
+    segments: (first row, rows, first state, states) of every request; rows of no segment (the text, say)
+    get nothing added. The table and the buffer of the attention's result belong to this object."""
+
+    def __init__(self, gpu: Gpu, shape: DitShape, *, rows: int, states: int, segments, kv_heads: int | None = None):
+        self.gpu, self.s, self.rows, self.states = gpu, shape, rows, states
+        self.kv_heads = kv_heads or shape.heads
+        if shape.heads % self.kv_heads:
+            raise ValueError("heads must divide by the number of key heads")
+        table = np.array(segments, np.int64).reshape(-1, 4)
+        first, count = table[:, 0], table[:, 1]
+        if (table < 0).any() or (first + count > rows).any() or (table[:, 2] + table[:, 3] > states).any():
+            raise ValueError("a segment reaches past the rows or the states")
+        order = np.argsort(first[count > 0], kind="stable")
+        starts, ends = first[count > 0][order], (first + count)[count > 0][order]
+        if (starts[1:] < ends[:-1]).any():
+            raise ValueError("the segments' rows overlap")
+        self.segment_count = len(table)
+        self.segments = gpu.u32(table.astype(np.uint32))
+        # rows of no segment are never written: they stay zero
+        self.heads = gpu.bf16(np.zeros(rows * shape.inner, np.uint16))
+        self.blocks: list[tuple[Tensor, Tensor]] = []
+
+    def add_block(self, encoder_states: Tensor, width: int, key_weight: Tensor, value_weight: Tensor,
+                  adapters: BlockAdapters | None = None, key_pair=None, value_pair=None) -> None:
+        """Keys and values of the next block from encoder_states [states][width]; `adapters` holds the
+        per-state map of the pairs, if there are any. Call inside a command."""
+        g, inner = self.gpu, self.kv_heads * self.s.head_dim
+        made = []
+        for weight, pair in ((key_weight, key_pair), (value_weight, value_pair)):
+            out = g.new(self.states * inner, BF16)
+            if adapters is not None and pair is not None:
+                adapters.project(g, pair, out, encoder_states, weight, self.states, width, inner)
+            else:
+                g.op("linear_bf16", out, encoder_states, weight, None, self.states, width, inner)
+            made.append(out)
+        self.blocks.append((made[0], made[1]))
+
+    def attend(self, block: int, query: Tensor, attention_heads: Tensor) -> None:
+        """attention_heads += attention of `query` to the states of `block`."""
+        g, s = self.gpu, self.s
+        key, value = self.blocks[block]
+        g.op("h3x_cross_sdpa_bf16", self.heads, query, key, value, self.segments, self.segment_count, self.rows, self.states,
+             s.heads, self.kv_heads, s.head_dim, s.scale)
+        g.op("add_bf16", attention_heads, attention_heads, self.heads, self.rows * s.inner)
+
+
 def block_tensor_shapes(s: DitShape, mod_rows: int) -> dict[str, int]:
     return {
         "norm1": s.hidden, "norm2": s.hidden,
@@ -125,6 +196,7 @@ class Dit:
         new = alloc or (lambda n: gpu.new(n, BF16))
         self.hidden = new(rows * s.hidden)
         self.mod_attention = new(rows * s.hidden)
+        self.mlp_fused = self.mlp_activated = None   # of an MLP with adapters, made by the first one
         self.push = world > 1 and hasattr(self.exchange, "setup")
         self.qkv = new(rows * max(3 * s.inner, s.hidden))   # also attention_heads and mod_mlp
         self.mod_mlp = self.qkv
@@ -169,11 +241,33 @@ class Dit:
              s.head_dim, ex.world)
 
     # ---------------------------------------------------------------- block
-    def run_block(self, w: BlockWeights, row_map: Tensor, rope_cos: Tensor, rope_sin: Tensor,
-                  adaln_ready: bool, next_w: BlockWeights | None) -> bool:
-        """One block; returns whether the next block's attention adaLN is already in
-        mod_attention (the cross-block fusion of h3_dit.c:2139-2177)."""
+    def _mlp(self, w: BlockWeights, adapters: BlockAdapters) -> None:
+        """The MLP with adapters on fc1, fc2 or both: where fc1 has some, SwiGLU follows as an op of its own
+        (the same rounding points as the fused form)."""
         g, s, rows = self.gpu, self.s, self.active_rows
+        if self.mlp_activated is None:
+            self.mlp_activated = g.new(self.rows_local * s.ffn, BF16)
+        if adapters.fc1 is not None:
+            if self.mlp_fused is None:
+                self.mlp_fused = g.new(self.rows_local * 2 * s.ffn, BF16)
+            adapters.project(g, adapters.fc1, self.mlp_fused, self.mod_mlp, w.fc1, rows, s.hidden, 2 * s.ffn)
+            g.op("swiglu_bf16", self.mlp_activated, self.mlp_fused, rows, s.ffn)
+        else:
+            g.op("h3x_linear_swiglu_bf16", self.mlp_activated, self.mod_mlp, w.fc1, rows, s.hidden, s.ffn)
+        if adapters.fc2 is not None:
+            adapters.project(g, adapters.fc2, self.attention_output, self.mlp_activated, w.fc2, rows, s.ffn, s.hidden)
+        else:
+            g.op("linear_bf16", self.attention_output, self.mlp_activated, w.fc2, None, rows, s.ffn, s.hidden)
+
+    def run_block(self, w: BlockWeights, row_map: Tensor, rope_cos: Tensor, rope_sin: Tensor,
+                  adaln_ready: bool, next_w: BlockWeights | None, adapters: BlockAdapters | None = None,
+                  conditioning: Conditioning | None = None, block: int = 0) -> bool:
+        """One block; returns whether the next block's attention adaLN is already in
+        mod_attention (the cross-block fusion of h3_dit.c:2139-2177). `adapters` go beside the block's
+        projections, `conditioning` adds its attention of block `block` to the heads."""
+        g, s, rows = self.gpu, self.s, self.active_rows
+        if (adapters is not None or conditioning is not None) and self.exchange.world != 1:
+            raise ValueError("adapters and conditioning are not combined with sequence parallelism")
         if not adaln_ready:
             g.op("adaln_bf16", self.mod_attention, self.hidden, w.norm1, w.modulation, row_map,
                  rows, s.hidden, s.slots, 0, 1, s.eps)
@@ -187,16 +281,29 @@ class Dit:
                  self.sequence, s.heads, s.head_dim, s.scale)
             ex.barrier()      # every head of this rank's rows has arrived
         else:
-            g.op("grouped_qkv_linear_rope_bf16", self.query, self.key, self.value, self.qkv,
-                 self.mod_attention, w.qkv, w.q_norm, w.k_norm, rope_cos, rope_sin, rows, s.hidden,
-                 s.heads, s.head_dim, s.rope_half, s.eps)
+            if adapters is not None and adapters.qkv is not None:
+                adapters.project(g, adapters.qkv, self.qkv, self.mod_attention, w.qkv, rows, s.hidden, 3 * s.inner)
+                g.op("grouped_qkv_rope_bf16", self.query, self.key, self.value, self.qkv, w.q_norm, w.k_norm, rope_cos,
+                     rope_sin, rows, s.heads, s.head_dim, s.rope_half, s.eps)
+            else:
+                g.op("grouped_qkv_linear_rope_bf16", self.query, self.key, self.value, self.qkv,
+                     self.mod_attention, w.qkv, w.q_norm, w.k_norm, rope_cos, rope_sin, rows, s.hidden,
+                     s.heads, s.head_dim, s.rope_half, s.eps)
             self._attention()
-        g.op("linear_bf16", self.attention_output, self.attention_heads, w.out, None, rows,
-             s.inner, s.hidden)
+            if conditioning is not None:
+                conditioning.attend(block, self.query, self.attention_heads)
+        if adapters is not None and adapters.out is not None:
+            adapters.project(g, adapters.out, self.attention_output, self.attention_heads, w.out, rows, s.inner, s.hidden)
+        else:
+            g.op("linear_bf16", self.attention_output, self.attention_heads, w.out, None, rows,
+                 s.inner, s.hidden)
         g.op("gate_adaln_bf16", self.hidden, self.mod_mlp, self.hidden, self.attention_output,
              w.norm2, w.modulation, w.modulation, row_map, rows, s.hidden, s.slots, 2, 3, 4, s.eps)
-        g.op("mlp_bf16", self.attention_output, self.mod_mlp, w.fc1, w.fc2, rows, s.hidden, s.ffn,
-             s.hidden)
+        if adapters is not None and (adapters.fc1 is not None or adapters.fc2 is not None):
+            self._mlp(w, adapters)
+        else:
+            g.op("mlp_bf16", self.attention_output, self.mod_mlp, w.fc1, w.fc2, rows, s.hidden, s.ffn,
+                 s.hidden)
         if next_w is not None:
             g.op("gate_adaln_bf16", self.hidden, self.mod_attention, self.hidden,
                  self.attention_output, next_w.norm1, w.modulation, next_w.modulation, row_map,
@@ -208,13 +315,22 @@ class Dit:
 
     def run_blocks(self, blocks: list[BlockWeights], row_map: Tensor, rope_cos: Tensor,
                    rope_sin: Tensor, reduction: "TokenReduction | None" = None,
-                   reduced_row_map: Tensor | None = None, fused_boundaries: bool = True) -> None:
+                   reduced_row_map: Tensor | None = None, fused_boundaries: bool = True,
+                   adapters: "list[BlockAdapters | None] | None" = None,
+                   conditioning: Conditioning | None = None) -> None:
         """All blocks. With `reduction`, blocks [begin, end) run on the pooled token grid
         (h3_dit.c:2316-2345): pool before block `begin`, expand before block `end` (or after the
         last block); the cross-block adaLN fusion is not carried over either boundary. With
         fused_boundaries (the reference's default) the pool / expand kernel also applies the
-        attention adaLN of the block that follows."""
+        attention adaLN of the block that follows. `adapters` has one entry per block; neither they nor
+        `conditioning` are combined with a reduction, whose rows are others."""
         red = reduction
+        if red is not None and (adapters is not None or conditioning is not None):
+            raise ValueError("adapters and conditioning are not combined with token reduction")
+        if adapters is not None and len(adapters) != len(blocks):
+            raise ValueError("adapters must have one entry per block")
+        if conditioning is not None and (len(conditioning.blocks) < len(blocks) or conditioning.rows != self.rows_local):
+            raise ValueError("conditioning must have these rows and keys and values for every block")
         if red is not None and self.exchange.world != 1:
             raise ValueError("token reduction is not combined with sequence parallelism")
         ready = False
@@ -228,7 +344,8 @@ class Dit:
             if red is not None and red.active:
                 ready = self.run_block(w, reduced_row_map, red.rope_cos, red.rope_sin, ready, nxt)
             else:
-                ready = self.run_block(w, row_map, rope_cos, rope_sin, ready, nxt)
+                ready = self.run_block(w, row_map, rope_cos, rope_sin, ready, nxt,
+                                       adapters[i] if adapters is not None else None, conditioning, i)
             if i == int(len(blocks) * 0.6):
                 self.gpu.flush()     # the reference's mid-step command split (h3_dit.c:2403-2406)
         if red is not None and red.active:
@@ -361,6 +478,8 @@ class DenoiseStep:
         self.final_weight, self.final_bias = final_weight, final_bias
         self.row_map, self.final_row_map = row_map, final_row_map
         self.rope_cos, self.rope_sin = rope_cos, rope_sin
+        self.adapters: list[BlockAdapters | None] | None = None      # one entry per block
+        self.conditioning: Conditioning | None = None
         g, s = dit.gpu, dit.s
         self.latent = g.new(max(1, video_rows) * s.video_patch, F32)       # patchified video rows
         self.velocity = g.new(max(1, video_rows) * s.video_patch, BF16)
@@ -375,7 +494,8 @@ class DenoiseStep:
         if self.video_rows:
             g.op("patch_linear_bf16_offset", d.hidden, self.text_rows * s.hidden, self.latent, 0,
                  self.patch_weight, self.patch_bias, self.video_rows, s.video_patch, s.hidden)
-        d.run_blocks(self.blocks, self.row_map, self.rope_cos, self.rope_sin)
+        d.run_blocks(self.blocks, self.row_map, self.rope_cos, self.rope_sin, adapters=self.adapters,
+                     conditioning=self.conditioning)
         if self.video_rows:
             g.op("adaln_linear_bf16", self.velocity, self.inverse, d.hidden,
                  self.text_rows * s.hidden, self.final_norm, self.final_modulation,
