@@ -300,6 +300,7 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     volatile float *xchg = reinterpret_cast<volatile float *>(ct_smem_raw + (bars - base) + CT_BARS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long budget = args.wait_cycles;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      /* the merge, which waits for this launch's end */
     if ((base & 1023u) != 0) {       /* swizzled tiles need 1024-byte alignment */
         if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_ATTN_TIMEOUT));
         return;
@@ -701,40 +702,63 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 }
 
 /* out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits in order, one warp per (row, head);
- * rows of no segment are left alone. */
+ * rows of no segment are left alone. 32 splits at a time: their statistics one per lane, their rows loaded
+ * eight ahead (one after the other they cost a memory latency each: 20 us for 32). */
 template <int D>
 __global__ void __launch_bounds__(256)
 h3b_cross_merge(const CrossArgs args) {
-    const size_t unit = (size_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (unit >= size_t(args.query_rows) * args.heads) return;
+    using Vector = std::conditional_t<D == 128, float4, float2>;
+    constexpr int PER = D / 32;
+    const size_t unit = (size_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5, all = size_t(args.query_rows) * args.heads;
     const uint32_t lane = threadIdx.x & 31, row = uint32_t(unit / args.heads);
-    bool found = !args.segments;
-    for (uint32_t i = lane; !found && i < args.segment_count; i += 32) {
+    /* the segment table is the caller's: no launch of this call writes it */
+    bool found = !args.segments && unit < all;
+    for (uint32_t i = lane; args.segments && unit < all && !found && i < args.segment_count; i += 32) {
         const Segment s = load_segment(args.segments, i, args.query_rows, args.key_rows);
         found = row - s.q0 < s.queries;
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");      /* every warp: this launch does not end before the one in front */
     if (!__any_sync(0xffffffffu, found)) return;
-    const size_t stride = size_t(args.query_rows) * args.heads;
-    float m = -INFINITY;
-    for (uint32_t s = 0; s < args.splits; s++) {
-        const float part = args.partial_ml[(s * stride + unit) * 2];
-        if (part > m || part != part) m = part;
+    float most = -INFINITY;
+    bool nan = false;
+    for (uint32_t s = lane; s < args.splits; s += 32) {
+        const float m = args.partial_ml[(s * all + unit) * 2];
+        most = fmaxf(most, m);
+        nan = nan || m != m;
     }
-    float sum = 0.0f, o[D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) o[i] = 0.0f;
-    for (uint32_t s = 0; s < args.splits; s++) {
-        const float2 ml = *reinterpret_cast<const float2 *>(args.partial_ml + (s * stride + unit) * 2);
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;       /* nothing attended: its O was not written */
-        const float weight = ct_exp2(ml.x - m);
-        sum = fmaf(ml.y, weight, sum);
-        const float *src = args.partial_o + (s * stride + unit) * D;
+    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (__any_sync(0xffffffffu, nan)) most = NAN;
+    float sum = 0.0f, o[PER];
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) o[i] = fmaf(src[lane + 32 * i], weight, o[i]);
+    for (int i = 0; i < PER; i++) o[i] = 0.0f;
+    for (uint32_t s0 = 0; s0 < args.splits; s0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (s0 + lane < args.splits) ml = *reinterpret_cast<const float2 *>(args.partial_ml + ((s0 + lane) * all + unit) * 2);
+        /* a part that attended nothing has no rows written */
+        const bool used = !(ml.x == -INFINITY && ml.y == 0.0f);
+        const float weight = used ? ct_exp2(ml.x - most) : 0.0f;
+        float part = used ? ml.y * weight : 0.0f;
+#pragma unroll
+        for (int q = 16; q; q >>= 1) part += __shfl_xor_sync(0xffffffffu, part, q);
+        sum += part;
+        const uint32_t used_mask = __ballot_sync(0xffffffffu, used), count = min(32u, args.splits - s0);
+#pragma unroll 8
+        for (uint32_t s = 0; s < count; s++) {
+            const Vector v = reinterpret_cast<const Vector *>(args.partial_o + ((s0 + s) * all + unit) * D)[lane];
+            const float w = __shfl_sync(0xffffffffu, weight, s);
+            if (used_mask >> s & 1u) {
+#pragma unroll
+                for (int i = 0; i < PER; i++) o[i] = fmaf(reinterpret_cast<const float *>(&v)[i], w, o[i]);
+            }
+        }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint32_t packed[PER / 2];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) args.out[unit * D + lane + 32 * i] = to_bf16(o[i] * inv);
+    for (int i = 0; i < PER / 2; i++) packed[i] = pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
+#pragma unroll
+    for (int i = 0; i < PER / 2; i++) reinterpret_cast<uint32_t *>(args.out + unit * D)[lane * (PER / 2) + i] = packed[i];
 }
 
 /* [rows][heads][D] BF16 as a 3-D tensor (dim, head, row); box = box_dims (64 or 32, one swizzled line) x
@@ -787,13 +811,16 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
     const uint64_t per_item = uint64_t(GROUPS) * CT >> args.pack_log2;
     uint64_t units = (args.query_rows / per_item + args.segment_count) * args.head_units;
     const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2), tiles = (args.key_rows + CT - 1) / CT;
-    /* The keys of a unit are split where the units alone leave SMs idle. Few rows: up to three units per
-     * resident CTA, which evens out segments of different lengths (four single rows over 512, 77, 2,048
-     * and 1 keys x 56 heads: 40 us unsplit, 34 in two, 30 in four, 31 in eight parts). Many rows: one
-     * round of CTAs, two key tiles or more each, since every part writes its rows in F32. */
+    /* The keys of a unit are split where the units alone leave SMs idle. One group: up to three units per resident
+     * CTA, which evens out segments of different lengths (four single rows over 512, 77, 2,048 and 1 keys x
+     * 56 heads: 40 us unsplit, 34 in two, 30 in four, 31 in eight parts). Two groups: one round of CTAs, two key
+     * tiles or more each. Every part writes its rows in F32 and they are read again: no more of that than
+     * there is to read of keys and values (1,000 rows, 16 heads on 2, 700 keys: 26 us in two parts, 19 unsplit). */
     uint64_t splits = GROUPS == 1 ? (3 * resident + units - 1) / units : resident / units;
     const uint64_t most = GROUPS == 1 ? tiles : tiles / 2;
+    const uint64_t worth = uint64_t(args.key_rows) * args.kv_heads / (uint64_t(args.query_rows) * args.heads * 2);
     splits = splits > most ? most : splits;
+    splits = splits > worth ? worth : splits;
     args.splits = splits < 1 ? 1 : uint32_t(splits);
     units *= args.splits;
     if (units > 0xffffffffull - 2 * resident) return h3b_fail(gpu, "cross attention has too many tiles");
@@ -810,7 +837,16 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
     h3b_cross_tc<D, GROUPS><<<grid, ct_threads<GROUPS>(), ct_smem<D, GROUPS>(), gpu->stream>>>(map_q, map_k, map_v, map_out, args);
     if (args.splits > 1) {
         const size_t warps = size_t(args.query_rows) * args.heads;
-        h3b_cross_merge<D><<<unsigned((warps + 7) / 8), 256, 0, gpu->stream>>>(args);
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(unsigned((warps + 7) / 8));
+        config.blockDim = dim3(256);
+        config.stream = gpu->stream;
+        cudaLaunchAttribute attribute;
+        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute.val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        cudaLaunchKernelEx(&config, h3b_cross_merge<D>, args);      /* an error is reported by h3b_launched */
     }
     return h3b_launched(gpu, "cross_sdpa_bf16", H3B_SDPA);
 }
@@ -873,7 +909,11 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
         args.head_units = heads / args.pack;
         args.units_per_kv = group / args.pack;
         args.scale_log2 = scale * 1.4426950408889634f;
-        const bool few = query_rows <= uint64_t(segment_count) * (CT >> args.pack_log2);
+        /* One group per CTA, two CTAs per SM: where segments hold a tile of rows or less on average, and where
+         * units of two tiles would leave more than half of the SMs idle (300 rows x 32 heads on 8, 300 keys,
+         * head_dim 64: 10.6 against 12.4 us; 1,664 x 24 heads x 257 keys, which fills them: 22.8 against 22.6). */
+        const uint64_t tile_rows = CT >> args.pack_log2, pairs = (query_rows / (2 * tile_rows) + segment_count) * args.head_units;
+        const bool few = query_rows <= segment_count * tile_rows || 2 * pairs <= uint64_t(gpu->sm_count);
         if (few) return head_dim == 128 ? ct_launch<128, 1>(gpu, args, q, k, v) : ct_launch<64, 1>(gpu, args, q, k, v);
         return head_dim == 128 ? ct_launch<128, 2>(gpu, args, q, k, v) : ct_launch<64, 2>(gpu, args, q, k, v);
     }
