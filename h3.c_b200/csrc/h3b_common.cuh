@@ -167,7 +167,7 @@ void *h3b_workspace(h3_gpu *gpu, size_t bytes);
 /* Scratch of one call of the adapter and conditioning operators: the context's workspace, or, while
  * the stream is being captured, memory that belongs to the graph (an allocation node, freed by a node
  * behind the call's kernels), so that no two graphs and no later growth of the workspace can touch
- * it. Null on failure; release goes behind the last launch that uses the block. */
+ * it. Null on failure and for no bytes; release goes behind the last launch that uses the block. */
 struct h3b_scratch {
     h3_gpu *gpu;
     void *data = nullptr;
@@ -175,8 +175,9 @@ struct h3b_scratch {
     h3b_scratch(h3_gpu *context, size_t bytes) : gpu(context) {
         cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
         captured = cudaStreamIsCapturing(gpu->stream, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+        if (!bytes) return;
         if (!captured) { data = h3b_workspace(gpu, bytes); return; }
-        if (cudaMallocAsync(&data, bytes ? bytes : 1, gpu->stream) != cudaSuccess) { cudaGetLastError(); data = nullptr; }
+        if (cudaMallocAsync(&data, bytes, gpu->stream) != cudaSuccess) { cudaGetLastError(); data = nullptr; }
     }
     ~h3b_scratch() { if (captured && data) cudaFreeAsync(data, gpu->stream); }
     h3b_scratch(const h3b_scratch &) = delete;

@@ -48,7 +48,7 @@ h3b_lora_simt(const uint16_t *x, const uint16_t *w, const uint16_t *bias, const 
     __shared__ float xs[16][65];
     __shared__ float ws[16][65];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const uint32_t row0 = blockIdx.y * 64, col0 = blockIdx.x * 64;
+    const uint32_t columns = uint32_t((uint64_t(n) + 63) / 64), row0 = blockIdx.x / columns * 64, col0 = blockIdx.x % columns * 64;
     float acc[4][4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -120,8 +120,10 @@ struct Ring {
     uint32_t stage0, full, empty, done, info, holder;
     volatile int *stop;
 };
-/* addresses, and (thread 0) the barriers: `arrivals` per full barrier */
-__device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, int *stop_flag, uint32_t arrivals) {
+/* addresses, and (thread 0) the barriers: `arrivals` per full barrier. `let_next`: the launch behind this one, which may
+ * begin early, does so when every CTA has its tensor memory: none can wait for columns of a CTA that waits
+ * for this launch. */
+__device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, int *stop_flag, uint32_t arrivals, bool let_next) {
     Ring r;
     r.stage0 = (smem_u32(raw) + 1023u) & ~1023u;
     r.full = r.stage0 + args.stages * args.stage_bytes;
@@ -140,7 +142,10 @@ __device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, i
         mbar_init(r.info, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (threadIdx.x >> 5 == 1) tmem_alloc(r.holder, args.tmem_columns);
+    if (threadIdx.x >> 5 == 1) {
+        tmem_alloc(r.holder, args.tmem_columns);
+        if (let_next) h3b_let_next_launch();
+    }
     return r;
 }
 /* behind the block barrier that follows ring_begin: the accumulator's address */
@@ -216,7 +221,7 @@ __device__ __forceinline__ void publish_entries(const Entries &s, const h3b_lora
 struct DownArgs {
     h3b_lora_task task;
     RingArgs ring;
-    uint32_t k_blocks, rank16, group;        /* columns per entry (rank rounded up to 16); entries per cluster */
+    uint32_t k_blocks, rank16, group;        /* columns per entry (rank rounded up to 16); entries at a time */
 };
 __global__ void __launch_bounds__(LR_THREADS)
 h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_down,
@@ -230,8 +235,7 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = gridDim.x, part = blockIdx.x, row0 = blockIdx.y * LR_M, tile = row0 / task.tile_rows;
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
-    h3b_let_next_launch();
-    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 2);
+    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 2, true);
     const uint32_t early = blockIdx.z == 0 ? min(args.ring.stages, kb1 - kb0) : 0;
     if (threadIdx.x == 0)
         for (uint32_t i = 0; i < early; i++) {
@@ -239,7 +243,6 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             tma_load_2d(ring.stage0 + i * args.ring.stage_bytes, &map_x, ring.full + 8 * i, int((kb0 + i) * LR_K), int(row0));
         }
     const uint32_t count = find_entries(found, task, tile);
-    const uint32_t e0 = blockIdx.z * args.group, e1 = min(count, e0 + args.group);
     if (blockIdx.z == 0 && part == 0 && row0 == tile * task.tile_rows) publish_entries(found, task, tile, count);
     if (threadIdx.x < LR_M) {
         const uint32_t a = adapter_of(task, row0 + threadIdx.x);
@@ -250,105 +253,110 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ring_tmem(ring);
-    const bool active = e0 < e1;                         /* the same in the whole cluster */
-    const uint32_t columns = (e1 - e0) * args.rank16;
-    if (!active) {
+    if (count == 0 && threadIdx.x == 0)
         /* nothing to compute; copies that went out have to land before the CTA leaves */
-        if (threadIdx.x == 0)
-            for (uint32_t i = 0; i < early; i++) {
-                mbar_arrive(ring.full + 8 * i);
-                mbar_wait(ring.full + 8 * i, 0, ring.stop, args.ring.wait_cycles);
-            }
-    } else if (warp == 0) {
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            for (uint32_t kb = kb0; kb < kb1; kb++) {
-                const uint32_t bar = ring.full + 8 * stage, dst = ring.stage0 + stage * args.ring.stage_bytes;
-                if (kb - kb0 >= early) {
-                    if (!mbar_wait(ring.empty + 8 * stage, phase ^ 1, ring.stop, args.ring.wait_cycles)) break;
-                    mbar_expect_tx(bar, LR_A_BYTES);
-                    tma_load_2d(dst, &map_x, bar, int(kb * LR_K), int(row0));
+        for (uint32_t i = 0; i < early; i++) {
+            mbar_arrive(ring.full + 8 * i);
+            mbar_wait(ring.full + 8 * i, 0, ring.stop, args.ring.wait_cycles);
+        }
+    /* Groups of entries blockIdx.z, blockIdx.z + gridDim.z, ...: as many turns in every CTA of the cluster, whatever
+     * any of them runs into. Stages and phases count on in the two roles that use them. */
+    uint32_t stage = 0, phase = 0, turn = 0;
+    for (uint32_t e0 = blockIdx.z * args.group; e0 < count; e0 += gridDim.z * args.group, turn++) {
+        const uint32_t e1 = min(count, e0 + args.group), columns = (e1 - e0) * args.rank16;
+        if (warp == 0) {
+            if (lane == 0) {
+                for (uint32_t kb = kb0; kb < kb1; kb++) {
+                    const uint32_t bar = ring.full + 8 * stage, dst = ring.stage0 + stage * args.ring.stage_bytes;
+                    if (turn || kb - kb0 >= early) {
+                        if (!mbar_wait(ring.empty + 8 * stage, phase ^ 1, ring.stop, args.ring.wait_cycles)) break;
+                        mbar_expect_tx(bar, LR_A_BYTES);
+                        tma_load_2d(dst, &map_x, bar, int(kb * LR_K), int(row0));
+                    }
+                    mbar_expect_tx(bar, columns * LR_K * 2);
+                    for (uint32_t e = e0; e < e1; e++)
+                        tma_load_2d(dst + LR_A_BYTES + (e - e0) * args.rank16 * LR_K * 2, &map_down, bar, int(kb * LR_K),
+                                    int(found.adapter[e] * task.rank));
+                    if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
                 }
-                mbar_expect_tx(bar, columns * LR_K * 2);
-                for (uint32_t e = e0; e < e1; e++)
-                    tma_load_2d(dst + LR_A_BYTES + (e - e0) * args.rank16 * LR_K * 2, &map_down, bar, int(kb * LR_K),
-                                int(found.adapter[e] * task.rank));
+            }
+        } else if (warp == 1) {
+            const uint32_t leader = lane == 0, idesc = instruction_desc(LR_M, int(columns));
+            bool alive = true;
+            for (uint32_t kb = kb0; kb < kb1; kb++) {
+                alive = __all_sync(0xffffffffu, mbar_wait(ring.full + 8 * stage, phase, ring.stop, args.ring.wait_cycles));
+                if (!alive) break;
+                tc_fence_after();
+                const uint32_t a_lo = desc_lo_kmajor(ring.stage0 + stage * args.ring.stage_bytes);
+                const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4);
+                if (kb == kb0) umma_ss<false>(tmem, a_lo, b_lo, idesc, leader);
+                else umma_ss<true>(tmem, a_lo, b_lo, idesc, leader);
+#pragma unroll
+                for (int k = 1; k < LR_K / 16; k++) umma_ss<true>(tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
+                umma_commit_if(ring.empty + 8 * stage, leader);
                 if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
             }
-        }
-    } else if (warp == 1) {
-        const uint32_t leader = lane == 0, idesc = instruction_desc(LR_M, int(columns));
-        uint32_t stage = 0, phase = 0;
-        bool alive = true;
-        for (uint32_t kb = kb0; kb < kb1; kb++) {
-            alive = __all_sync(0xffffffffu, mbar_wait(ring.full + 8 * stage, phase, ring.stop, args.ring.wait_cycles));
-            if (!alive) break;
-            tc_fence_after();
-            const uint32_t a_lo = desc_lo_kmajor(ring.stage0 + stage * args.ring.stage_bytes);
-            const uint32_t b_lo = a_lo + (LR_A_BYTES >> 4);
-            if (kb == kb0) umma_ss<false>(tmem, a_lo, b_lo, idesc, leader);
-            else umma_ss<true>(tmem, a_lo, b_lo, idesc, leader);
+            if (alive) umma_commit_if(ring.done, leader);
+        } else {
+            /* accumulator -> this CTA's shared memory, [row][columns] F32 with 16-byte pieces XOR-swizzled by row
+             * (every copy and product of this CTA is complete, the stages are free) */
+            const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
+            if (__all_sync(0xffffffffu, mbar_wait(ring.done, turn & 1u, ring.stop, args.ring.wait_cycles))) {
+                tc_fence_after();
+                for (uint32_t c = 0; c < columns; c += 16) {
+                    uint32_t v[16];
+                    asm volatile(
+                        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                        : "r"(tmem + ((quarter * 32) << 16) + c) : "memory");
+                    tmem_ld_wait();
 #pragma unroll
-            for (int k = 1; k < LR_K / 16; k++) umma_ss<true>(tmem, a_lo + 2 * k, b_lo + 2 * k, idesc, leader);
-            umma_commit_if(ring.empty + 8 * stage, leader);
-            if (++stage == args.ring.stages) { stage = 0; phase ^= 1; }
-        }
-        if (alive) umma_commit_if(ring.done, leader);
-    } else {
-        /* accumulator -> this CTA's shared memory, [row][columns] F32 with 16-byte pieces XOR-swizzled by row
-         * (every copy and product of this CTA is complete, the stages are free) */
-        const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
-        if (__all_sync(0xffffffffu, mbar_wait(ring.done, 0, ring.stop, args.ring.wait_cycles))) {
-            tc_fence_after();
-            for (uint32_t c = 0; c < columns; c += 16) {
-                uint32_t v[16];
-                asm volatile(
-                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                    : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                      "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                    : "r"(tmem + ((quarter * 32) << 16) + c) : "memory");
-                tmem_ld_wait();
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    const uint32_t piece = (c / 4 + i) ^ (row & 3);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ring.stage0 + (row * columns + piece * 4) * 4),
-                                 "r"(v[4 * i]), "r"(v[4 * i + 1]), "r"(v[4 * i + 2]), "r"(v[4 * i + 3]) : "memory");
+                    for (uint32_t i = 0; i < 4; i++) {
+                        const uint32_t piece = (c / 4 + i) ^ (row & 3);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(ring.stage0 + (row * columns + piece * 4) * 4),
+                                     "r"(v[4 * i]), "r"(v[4 * i + 1]), "r"(v[4 * i + 2]), "r"(v[4 * i + 3]) : "memory");
+                    }
                 }
+                tc_fence_before();
             }
         }
-    }
-    __syncwarp();
-    if (active) cluster_sync_all();
-    if (active && !*ring.stop) {
-        /* rows part, part + split, ...: the row's own columns of all CTAs, scaled and rounded; zeros for the
-         * entries that are not its own */
-        const uint32_t mine = (LR_M - part + split - 1) / split, pieces = task.rank8 / 4;
-        const uint32_t items = mine * (e1 - e0) * pieces;
-        for (uint32_t i = threadIdx.x; i < items; i += LR_THREADS) {
-            const uint32_t j = i % pieces * 4, e = e0 + i / pieces % (e1 - e0), r = part + i / pieces / (e1 - e0) * split;
-            if (row0 + r >= task.rows) continue;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (own[r] == e) {
-                const uint32_t c = (e - e0) * args.rank16 + j;
-                const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4) * 4;
-                for (uint32_t p = 0; p < split; p++) {
-                    float4 x;
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_map(at, p)) : "memory");
-                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        __syncwarp();
+        cluster_sync_all();
+        if (!*ring.stop) {
+            /* rows part, part + split, ...: the row's own columns of all CTAs, scaled and rounded; zeros for the
+             * entries that are not its own */
+            const uint32_t mine = (LR_M - part + split - 1) / split, pieces = task.rank8 / 4;
+            const uint32_t items = mine * (e1 - e0) * pieces;
+            for (uint32_t i = threadIdx.x; i < items; i += LR_THREADS) {
+                const uint32_t j = i % pieces * 4, e = e0 + i / pieces % (e1 - e0), r = part + i / pieces / (e1 - e0) * split;
+                if (row0 + r >= task.rows) continue;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (own[r] == e) {
+                    const uint32_t c = (e - e0) * args.rank16 + j;
+                    const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4) * 4;
+                    for (uint32_t p = 0; p < split; p++) {
+                        float4 x;
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_map(at, p)) : "memory");
+                        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+                    }
+                    const float s = own_scale[r];
+                    v.x = j < task.rank ? v.x * s : 0.0f;
+                    v.y = j + 1 < task.rank ? v.y * s : 0.0f;
+                    v.z = j + 2 < task.rank ? v.z * s : 0.0f;
+                    v.w = j + 3 < task.rank ? v.w * s : 0.0f;
                 }
-                const float s = own_scale[r];
-                v.x = j < task.rank ? v.x * s : 0.0f;
-                v.y = j + 1 < task.rank ? v.y * s : 0.0f;
-                v.z = j + 2 < task.rank ? v.z * s : 0.0f;
-                v.w = j + 3 < task.rank ? v.w * s : 0.0f;
+                *reinterpret_cast<uint2 *>(task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + (row0 + r) % task.tile_rows) * task.rank8 + j) =
+                    make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
             }
-            *reinterpret_cast<uint2 *>(task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + (row0 + r) % task.tile_rows) * task.rank8 + j) =
-                make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
         }
+        /* nobody leaves, or loads over its shared memory, while that may be read */
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        cluster_sync_all();
+        tc_fence_after();
     }
-    if (active) cluster_sync_all();      /* nobody leaves while its shared memory may be read */
     ring_close(args.ring, ring, tmem);
     h3b_wait_for_launch();               /* the padded up rows, where a launch in front writes them: done before this one is */
 }
@@ -413,7 +421,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const uint32_t row0 = tile * task.tile_rows, live = min(task.tile_rows, task.rows - row0);
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
     const uint32_t b_bytes = task.tile_rows * LR_K * 2;
-    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1);
+    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1, false);
     __shared__ uint32_t entries;
     __shared__ uint16_t adapter[LR_M];
     tc_fence_before();
@@ -672,8 +680,9 @@ uint32_t split_for(h3_gpu *gpu, Kernel *kernel, size_t smem, uint32_t per_sm, ui
     return 1;
 }
 
-/* Rows [0, task.rows) on the tensor cores; scratch as laid out by the caller. */
-int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool captured) {
+/* Rows [0, task.rows) on the tensor cores; scratch as laid out by the caller. `behind`: the launch that pads up is
+ * in front on the stream. */
+int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool behind, bool captured) {
     const uint32_t k_blocks = (task.k + LR_K - 1) / LR_K;
     const uint32_t tiles = (task.rows + task.tile_rows - 1) / task.tile_rows, row_blocks = (task.rows + LR_M - 1) / LR_M;
     CUtensorMap map_x, map_down;
@@ -694,17 +703,20 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
     const uint32_t want = two ? 106 << 10 : 200 << 10;
     down.ring.stages = want / down.ring.stage_bytes;
     if (down.ring.stages > uint32_t(LR_STAGES)) down.ring.stages = LR_STAGES;
-    const uint32_t down_split = split_for(gpu, h3b_lora_down_tc, ring_smem(down.ring), two ? 2 : 1, row_blocks, k_blocks);
+    const uint32_t per_sm = two ? 2 : 1, down_split = split_for(gpu, h3b_lora_down_tc, ring_smem(down.ring), per_sm, row_blocks, k_blocks);
+    /* Groups of entries run side by side while all run in one round, and in turn beyond that: most tiles hold few of
+     * many adapters, and a CTA that finds nothing to do costs its set-up (6,400 rows, 5,376 -> 5,376, 4 of 256
+     * adapters of rank 64 occur: 302 us in turn, 534 with every group side by side; all of 64: 343, 398) */
+    const uint64_t room = per_sm * resident_clusters(gpu->device, h3b_lora_down_tc, down_split, ring_smem(down.ring)) / row_blocks;
+    const uint32_t side = groups < room ? groups : room < 1 ? 1 : uint32_t(room);
     if (!lora_map(&map_x, task.x, task.rows, task.k, LR_M) ||
         !lora_map(&map_down, task.down, uint64_t(task.adapters) * task.rank, task.k, down.rank16))
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
-    /* behind the launch that pads up, if there is one */
-    const bool behind = task.up8 != task.up;
     /* by warps while that reads the inputs a few times at most from L2 */
     if (few && task.rows <= uint32_t(LR_M) && uint64_t(task.rows) * task.rank <= 2048)
         launch_cluster(gpu, h3b_lora_down_few, dim3(task.rows, task.rank8 / LF_SUMS), 32 * LF_WARPS, 1, 0, behind, task);
     else
-        launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, groups), LR_THREADS, down_split, ring_smem(down.ring), behind,
+        launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, side), LR_THREADS, down_split, ring_smem(down.ring), behind,
                        map_x, map_down, down);
     if (cudaGetLastError() != cudaSuccess) return h3b_fail(gpu, "linear_lora_bf16: the low-rank rows cannot be launched");
     if (!few) {
@@ -773,7 +785,7 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
     uint16_t *y = h3b_ptr<uint16_t>(output);
 
     const bool aligned = h3b_aligned16(x) && h3b_aligned16(w) && (!b || h3b_aligned16(b)) && h3b_aligned16(d) && h3b_aligned16(u) && h3b_aligned16(y);
-    if (aligned && input_dim && input_dim % 8 == 0 && output_dim % 8 == 0 && !lora_env("H3B_NO_TENSOR_CORES") &&
+    if (aligned && input_dim && input_dim % 8 == 0 && output_dim % 8 == 0 && input_dim <= INT32_MAX && output_dim <= INT32_MAX && !lora_env("H3B_NO_TENSOR_CORES") &&
         double(rows) * output_dim * input_dim >= 32.0 * 256 * 256) {      /* tiny problems are latency bound either way */
         if (!lora_configure(gpu->device)) return h3b_fail(gpu, "cannot reserve shared memory for the adapter kernels");
         h3b_lora_task task = {};
@@ -794,7 +806,8 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
         /* room for every adapter in every tile; so many rows at a time that it stays within a gigabyte */
         const size_t tile_bytes = size_t(task.max_entries) * tile_rows * task.rank8 * 2;
         size_t chunk_tiles = (size_t(1) << 30) / tile_bytes;
-        const size_t all_tiles = (rows + tile_rows - 1) / tile_rows;
+        if (chunk_tiles > 32768) chunk_tiles = 32768;          /* 128-row blocks are counted in a grid's y */
+        const size_t all_tiles = (size_t(rows) + tile_rows - 1) / tile_rows;
         if (chunk_tiles > all_tiles) chunk_tiles = all_tiles;
         const size_t t_bytes = rounded(chunk_tiles * tile_bytes);
         const size_t up_bytes = task.rank8 == rank ? 0 : rounded(size_t(adapters) * output_dim * task.rank8 * 2);
@@ -818,16 +831,23 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
             part.x = x + row0 * input_dim;
             part.out = y + row0 * output_dim;
             part.row_adapter = map ? map + row0 : nullptr;
-            if (!lora_tensor_cores(gpu, part, few, scratch.captured)) return 0;
+            if (!lora_tensor_cores(gpu, part, few, up_bytes && !tile, scratch.captured)) return 0;
         }
         return h3b_launched(gpu, "linear_lora_bf16", kind);
     }
-    h3b_scratch scratch(gpu, size_t(rows) * rank * sizeof(float));
+    /* so many rows at a time that their low-rank rows stay within 256 MB and grids within their limits */
+    const size_t most = (size_t(1) << 26) / rank, chunk = rows < most ? rows : most;
+    h3b_scratch scratch(gpu, chunk * rank * sizeof(float));
     if (!scratch.data) return h3b_fail(gpu, "linear_lora_bf16: cannot allocate the low-rank rows");
     float *t = static_cast<float *>(scratch.data);
-    const size_t warps = size_t(rows) * rank;
-    h3b_lora_down_simt<<<unsigned((warps + 7) / 8), 256, 0, gpu->stream>>>(x, d, s, map, t, rows, input_dim, adapters, rank);
-    h3b_lora_simt<<<dim3((output_dim + 63) / 64, (rows + 63) / 64), 256, 0, gpu->stream>>>(
-        x, w, b, u, t, map, y, rows, input_dim, output_dim, adapters, rank);
+    for (size_t row0 = 0; row0 < rows; row0 += chunk) {
+        const uint32_t part = uint32_t(rows - row0 < chunk ? rows - row0 : chunk);
+        const uint32_t *part_map = map ? map + row0 : nullptr;
+        h3b_lora_down_simt<<<unsigned((size_t(part) * rank + 7) / 8), 256, 0, gpu->stream>>>(x + row0 * input_dim, d, s, part_map, t, part,
+                                                                                            input_dim, adapters, rank);
+        const size_t tiles = size_t((part + 63) / 64) * ((size_t(output_dim) + 63) / 64);
+        h3b_lora_simt<<<unsigned(tiles), 256, 0, gpu->stream>>>(x + row0 * input_dim, w, b, u, t, part_map, y + row0 * output_dim, part,
+                                                                input_dim, output_dim, adapters, rank);
+    }
     return h3b_launched(gpu, "linear_lora_bf16", kind);
 }

@@ -85,3 +85,20 @@ def test_block_with_adapters_and_conditioning(pkg, rows, text_rows, heads, kv_he
     without = o.dit_block(case.hidden, c, case.row_map, case.rope_cos, case.rope_sin, rows=rows, width=hidden, heads=heads,
                           head_dim=128, ffn=ffn, rope_half=48, round_p=1)
     assert_block_close(plain, without, "the plain block afterwards")
+
+
+def test_conditioning_without_requests_adds_nothing(pkg):
+    gpu = pkg.Gpu(0)
+    try:
+        shape = pkg.DitShape(hidden=64, heads=2, ffn=32, blocks=1)
+        cond = pkg.Conditioning(gpu, shape, rows=5, states=3, segments=[])
+        rng = np.random.default_rng(1)
+        query, heads = gpu.bf16(bits(rng, 5 * 256)), bits(rng, 5 * 256)
+        out = gpu.bf16(heads)
+        gpu.begin()
+        cond.add_block(gpu.bf16(bits(rng, 3, 32)), 32, gpu.bf16(bits(rng, 256, 32)), gpu.bf16(bits(rng, 256, 32)))
+        cond.attend(0, query, out)
+        gpu.submit()
+        assert np.array_equal(out.read(), heads)
+    finally:
+        gpu.close()

@@ -103,6 +103,43 @@ def test_model_sizes(gpu, pkg, rows, k, n, adapters, rank, kind):
     assert_within(case.run(gpu, pkg), *case.reference(), f"{case.sizes()}")
 
 
+@pytest.mark.parametrize("rows,k,n,adapters,rank,kind", [
+    (300, 328, 520, 256, 64, "each"), (700, 1024, 256, 1024, 16, "random"), (260, 512, 520, 40, 200, "each"),
+    (100, 512, 520, 100, 48, "each"), (2000, 512, 256, 300, 16, "runs")])
+def test_more_adapters_than_are_computed_side_by_side(gpu, pkg, rows, k, n, adapters, rank, kind):
+    case = Case(rows, k, n, adapters, rank, kind=kind)
+    assert_within(case.run(gpu, pkg), *case.reference(), f"{case.sizes()}")
+
+
+@pytest.mark.parametrize("rank", [256, 250])
+def test_low_rank_rows_beyond_a_gigabyte(gpu, pkg, rank):
+    """256 entries of 256 rows in every tile: the rows are taken in several passes."""
+    case = Case(9001, 64, 64, 256, rank, kind="random")
+    assert_within(case.run(gpu, pkg), *case.reference(), f"rank {rank}")
+
+
+@pytest.mark.parametrize("rows,k,n,rank", [(9_000_001, 8, 8, 8), (4_300_001, 3, 3, 2)])
+def test_more_rows_than_a_grid_dimension_holds(gpu, pkg, rows, k, n, rank):
+    """On the tensor cores and on the kernels for any shape; the input repeats a base block of rows."""
+    base = Case(1009, k, n, 3, rank, kind="random")
+    want, tol = base.reference()
+    tensors = base.tensors(gpu)
+    tensors[0].free()
+    tensors[6].free()
+    tensors[0] = gpu.bf16(np.resize(base.x, rows * k))
+    tensors[6] = gpu.u32(np.resize(base.map, rows))
+    out = gpu.bf16(np.full(rows * n, 0x7FC0, np.uint16))
+    gpu.begin()
+    gpu.op("h3x_linear_lora_bf16", out, *tensors, rows, k, n, 3, rank)
+    gpu.submit()
+    got = wide(out.read()).reshape(rows, n)
+    for t in [out, *tensors]:
+        t.free()
+    for row0 in range(0, rows, 1009):
+        count = min(1009, rows - row0)
+        assert (np.abs(got[row0:row0 + count] - want[:count]) <= tol[:count]).all(), row0
+
+
 @pytest.mark.parametrize("rows,k,n", [(5, 264, 272), (48, 512, 1024), (200, 512, 520), (400, 1024, 768)])
 def test_an_adapter_of_infinities_stays_with_its_own_rows(gpu, pkg, rows, k, n):
     """Rows of other adapters and rows without one are finite and right, whatever adapter 1 holds."""
@@ -210,8 +247,8 @@ def test_unaligned_tensors(gpu, pkg):
     assert_within(out.read(), *case.reference(), "unaligned")
 
 
-@pytest.mark.parametrize("rows", [3, 300])
-def test_on_another_stream_and_captured(pkg, rows):
+@pytest.mark.parametrize("rows,rank", [(3, 16), (300, 16), (3, 12), (300, 12)])
+def test_on_another_stream_and_captured(pkg, rows, rank):
     """The op on a caller's stream, captured twice into graphs whose replays use inputs written later;
     a larger call in between may grow the context's workspace."""
     import torch
@@ -219,7 +256,7 @@ def test_on_another_stream_and_captured(pkg, rows):
     stream = torch.cuda.Stream()
     try:
         gpu.set_stream(stream.cuda_stream)
-        cases = [Case(rows, 1024, 1024, 3, 16, kind="random", seed=s) for s in (1, 2)]
+        cases = [Case(rows, 1024, 1024, 3, rank, kind="random", seed=s) for s in (1, 2)]
         sets = [(c, c.tensors(gpu), gpu.new(rows * 1024, pkg.BF16)) for c in cases]
         big = Case(900, 1024, 520, 8, 128, kind="each")
         big_set = (big.tensors(gpu), gpu.new(900 * 520, pkg.BF16))
