@@ -1,7 +1,7 @@
 /* Cross attention: query rows of several requests to an encoder's states of other lengths.
  *
  * h3b_cross_tc (head_dim 64 and 128) runs on the tensor cores, described at its definition;
- * h3b_cross_merge joins its partial results where the keys of a segment are split. h3b_cross_simt takes
+ * h3b_cross_merge joins its partial results where the keys of a segment are cut into pieces. h3b_cross_simt takes
  * any head size, alignment and scale: one CTA per (query row, head) walks the keys of the row's segment
  * with the online softmax recurrence in F32.
  */
@@ -161,42 +161,51 @@ static_assert(2 * (ct_smem<128, 1>() + 1024) <= 233472, "two one-group CTAs per 
 struct CrossArgs {
     uint16_t *out;
     const uint32_t *segments;
-    float *partial_o, *partial_ml;       /* splits > 1: [split][query row][head][D], [split][query row][head][2] */
+    float *partial_o, *partial_ml;       /* segments in several pieces: [piece][query row][head][D], [piece][query row][head][2] */
     int *status;
     long long wait_cycles;
     uint32_t segment_count, query_rows, key_rows, heads, kv_heads;
     uint32_t pack, pack_log2, head_units;    /* head_units = heads / pack */
     uint32_t units_per_kv;                   /* head units that share a key head */
-    uint32_t splits;
-    uint32_t step_h, step_s, step_i;         /* the grid as (head unit, split, item) digits */
+    uint32_t per_piece;                      /* how the keys of a segment are cut: ct_pieces */
+    uint32_t step_h, step_i;                 /* the grid as (head unit, item) digits */
     uint32_t block_stores;                   /* whole tiles leave through map_out */
     float scale_log2;
 };
+
+/* The keys of a segment go to this many units, of about the same number of key tiles: tiles / length, rounded up. As
+ * the high half of a product with 2^31 / length, rounded down (2 tiles - 1 halves away from every multiple, so exact
+ * while tiles * length < 2^30, else a piece fewer): every cursor asks for every segment, and with a division 64
+ * segments of one row took 139 instead of 126 us. per_piece 0: one unit. */
+__device__ __forceinline__ uint32_t ct_pieces(uint32_t keys, uint32_t per_piece) {
+    return 1 + __umulhi(2 * ((max(keys, 1u) - 1) / CT) + 1, per_piece);
+}
 
 /* One work unit; every role walks the same units with a cursor of its own */
 struct CrossUnit {
     uint32_t q_row, rows;        /* first query row, live query rows (of all groups) */
     uint32_t head0, kv_head;
     uint32_t k_row, keys;        /* first key row of the range; keys of the segment from there on */
-    uint32_t steps, split;
+    uint32_t steps, piece;
+    bool cut;                    /* one of several pieces of the segment's keys */
     bool dirty;                  /* the last tile reaches rows that are not the segment's */
 };
 
 template <int GROUPS>
 struct CrossCursor {
-    uint32_t h, s, item;            /* the next unit: head unit (fastest), split, item (pair of tiles) */
+    uint32_t h, item;               /* the next unit: head unit (fastest), item (a piece of a pair of tiles) */
     uint32_t index, before, items;  /* the segment that item is looked for in, items in front of it, its items */
+    uint32_t pieces;
     Segment segment;
     __device__ __forceinline__ void enter(const CrossArgs &a) {
         segment = load_segment(a.segments, index, a.query_rows, a.key_rows);
         const uint32_t per_item = GROUPS * CT >> a.pack_log2;
-        items = (segment.queries + per_item - 1) >> ((GROUPS == 2 ? 8 : 7) - a.pack_log2);
+        pieces = ct_pieces(segment.keys, a.per_piece);
+        items = ((segment.queries + per_item - 1) >> ((GROUPS == 2 ? 8 : 7) - a.pack_log2)) * pieces;
     }
     __device__ __forceinline__ explicit CrossCursor(const CrossArgs &a) : index(0), before(0) {
         h = blockIdx.x % a.head_units;
-        const uint32_t rest = blockIdx.x / a.head_units;
-        s = rest % a.splits;
-        item = rest / a.splits;
+        item = blockIdx.x / a.head_units;
         enter(a);
     }
     __device__ __forceinline__ bool next(const CrossArgs &a, CrossUnit &u) {
@@ -205,27 +214,27 @@ struct CrossCursor {
             if (++index >= a.segment_count) return false;
             enter(a);
         }
-        const uint32_t tile_rows = CT >> a.pack_log2, first = (item - before) * GROUPS * tile_rows, left = segment.queries - first;
+        const uint32_t tiles = (segment.keys + CT - 1) / CT;
+        uint32_t at = item - before, t0 = 0, t1 = tiles;
+        u.cut = pieces > 1;
+        if (u.cut) {
+            u.piece = at % pieces;
+            at /= pieces;
+            t0 = uint32_t(uint64_t(u.piece) * tiles / pieces);
+            t1 = uint32_t(uint64_t(u.piece + 1) * tiles / pieces);
+        }
+        const uint32_t tile_rows = CT >> a.pack_log2, first = at * GROUPS * tile_rows, left = segment.queries - first;
         u.q_row = segment.q0 + first;
         u.rows = min(GROUPS * tile_rows, left);
         u.head0 = h << a.pack_log2;
         u.kv_head = a.units_per_kv == 1 ? h : h / a.units_per_kv;
-        u.split = s;
-        const uint32_t tiles = (segment.keys + CT - 1) / CT;
-        uint32_t t0 = 0, t1 = tiles;
-        if (a.splits > 1) {
-            t0 = uint32_t(uint64_t(s) * tiles / a.splits);
-            t1 = uint32_t(uint64_t(s + 1) * tiles / a.splits);
-        }
         u.k_row = segment.k0 + t0 * CT;
         u.keys = segment.keys - t0 * CT;
         u.steps = t1 - t0;
         u.dirty = t1 == tiles && (segment.keys & (CT - 1)) && segment.k0 + segment.keys < a.key_rows;
         h += a.step_h;
-        s += a.step_s;
         item += a.step_i;
-        if (h >= a.head_units) { h -= a.head_units; s++; }
-        if (s >= a.splits) { s -= a.splits; item++; }
+        if (h >= a.head_units) { h -= a.head_units; item++; }
         return true;
     }
 };
@@ -512,13 +521,10 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             auto unit_of_row = [&] { return size_t(q_row + row_in_tile) * args.heads + u.head0 + (local_row & (args.pack - 1)); };
             const uint32_t steps = u.steps;
             if (!steps) {
-                if (live && args.splits == 1) {            /* no keys: zeros */
+                if (live) {            /* no keys: zeros */
                     uint4 *dst = reinterpret_cast<uint4 *>(args.out + unit_of_row() * D + half * (D / 2));
 #pragma unroll
                     for (int i = 0; i < D / 16; i++) dst[i] = make_uint4(0, 0, 0, 0);
-                } else if (live && !half) {                /* a part that weighs nothing */
-                    *reinterpret_cast<float2 *>(args.partial_ml + (size_t(u.split) * args.query_rows * args.heads + unit_of_row()) * 2) =
-                        make_float2(-INFINITY, 0.0f);
                 }
                 have = cursor.next(args, u);
                 continue;
@@ -620,14 +626,15 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             if (!alive) break;
             sum += *my_x;
             const size_t unit = unit_of_row();
-            const uint32_t head0 = u.head0, split = u.split;
+            const uint32_t head0 = u.head0, piece = u.piece;
+            const bool cut = u.cut;
             have = cursor.next(args, u);
             alive = meet(__all_sync(0xffffffffu, mbar_wait(o_done + 8 * g, o_phase, stop, budget)));
             if (!alive) break;
             o_phase ^= 1;
             tc_fence_after();
-            if (args.splits > 1) {
-                const size_t at = size_t(split) * args.query_rows * args.heads + unit;
+            if (cut) {
+                const size_t at = size_t(piece) * args.query_rows * args.heads + unit;
                 if (live && !half) *reinterpret_cast<float2 *>(args.partial_ml + at * 2) = make_float2(reference, sum);
 #pragma unroll 1
                 for (int c = 0; c < D / 2; c += 32) {
@@ -701,8 +708,8 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     }
 }
 
-/* out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits in order, one warp per (row, head);
- * rows of no segment are left alone. 32 splits at a time: their statistics one per lane, their rows loaded
+/* out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over a segment's pieces s in order, one warp per (row, head);
+ * rows of no segment, and of segments in one piece, are left alone. 32 pieces at a time: their statistics one per lane, their rows loaded
  * eight ahead (one after the other they cost a memory latency each: 20 us for 32). */
 template <int D>
 __global__ void __launch_bounds__(256)
@@ -712,16 +719,18 @@ h3b_cross_merge(const CrossArgs args) {
     const size_t unit = (size_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5, all = size_t(args.query_rows) * args.heads;
     const uint32_t lane = threadIdx.x & 31, row = uint32_t(unit / args.heads);
     /* the segment table is the caller's: no launch of this call writes it */
-    bool found = !args.segments && unit < all;
-    for (uint32_t i = lane; args.segments && unit < all && !found && i < args.segment_count; i += 32) {
+    uint32_t pieces = 0;
+    if (!args.segments) pieces = unit < all ? ct_pieces(args.key_rows, args.per_piece) : 0;
+    for (uint32_t i = lane; args.segments && unit < all && i < args.segment_count; i += 32) {
         const Segment s = load_segment(args.segments, i, args.query_rows, args.key_rows);
-        found = row - s.q0 < s.queries;
+        if (row - s.q0 < s.queries) pieces = ct_pieces(s.keys, args.per_piece);
     }
+    pieces = __reduce_max_sync(0xffffffffu, pieces);
     asm volatile("griddepcontrol.wait;" ::: "memory");      /* every warp: this launch does not end before the one in front */
-    if (!__any_sync(0xffffffffu, found)) return;
+    if (pieces < 2) return;
     float most = -INFINITY;
     bool nan = false;
-    for (uint32_t s = lane; s < args.splits; s += 32) {
+    for (uint32_t s = lane; s < pieces; s += 32) {
         const float m = args.partial_ml[(s * all + unit) * 2];
         most = fmaxf(most, m);
         nan = nan || m != m;
@@ -732,9 +741,9 @@ h3b_cross_merge(const CrossArgs args) {
     float sum = 0.0f, o[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) o[i] = 0.0f;
-    for (uint32_t s0 = 0; s0 < args.splits; s0 += 32) {
+    for (uint32_t s0 = 0; s0 < pieces; s0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.0f);
-        if (s0 + lane < args.splits) ml = *reinterpret_cast<const float2 *>(args.partial_ml + ((s0 + lane) * all + unit) * 2);
+        if (s0 + lane < pieces) ml = *reinterpret_cast<const float2 *>(args.partial_ml + ((s0 + lane) * all + unit) * 2);
         /* a part that attended nothing has no rows written */
         const bool used = !(ml.x == -INFINITY && ml.y == 0.0f);
         const float weight = used ? ct_exp2(ml.x - most) : 0.0f;
@@ -742,7 +751,7 @@ h3b_cross_merge(const CrossArgs args) {
 #pragma unroll
         for (int q = 16; q; q >>= 1) part += __shfl_xor_sync(0xffffffffu, part, q);
         sum += part;
-        const uint32_t used_mask = __ballot_sync(0xffffffffu, used), count = min(32u, args.splits - s0);
+        const uint32_t used_mask = __ballot_sync(0xffffffffu, used), count = min(32u, pieces - s0);
 #pragma unroll 8
         for (uint32_t s = 0; s < count; s++) {
             const Vector v = reinterpret_cast<const Vector *>(args.partial_o + ((s0 + s) * all + unit) * D)[lane];
@@ -807,35 +816,49 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
         !ct_map(&map_k, k, args.key_rows, args.kv_heads, D, 64, 1, CT) ||
         !ct_map(&map_v, v, args.key_rows, args.kv_heads, D, 64, 1, CT))
         return h3b_fail(gpu, "cannot encode the cross attention tensor maps");
-    /* most units there can be: every segment may end in a part of a tile */
-    const uint64_t per_item = uint64_t(GROUPS) * CT >> args.pack_log2;
-    uint64_t units = (args.query_rows / per_item + args.segment_count) * args.head_units;
-    const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2), tiles = (args.key_rows + CT - 1) / CT;
-    /* The keys of a unit are split where the units alone leave SMs idle. One group: up to three units per resident
-     * CTA, which evens out segments of different lengths (four single rows over 512, 77, 2,048 and 1 keys x
-     * 56 heads: 40 us unsplit, 34 in two, 30 in four, 31 in eight parts). Two groups: one round of CTAs, two key
-     * tiles or more each. Every part writes its rows in F32 and they are read again: no more of that than
-     * there is to read of keys and values (1,000 rows, 16 heads on 2, 700 keys: 26 us in two parts, 19 unsplit). */
-    uint64_t splits = GROUPS == 1 ? (3 * resident + units - 1) / units : resident / units;
-    const uint64_t most = GROUPS == 1 ? tiles : tiles / 2;
+    const uint64_t per_item = uint64_t(GROUPS) * CT >> args.pack_log2, tiles = (uint64_t(args.key_rows) + CT - 1) / CT;
+    const uint64_t resident = uint64_t(gpu->sm_count) * (GROUPS == 2 ? 1 : 2);
+    /* The keys of a segment are cut into pieces of about so many key tiles. If rows and keys are spread evenly over the
+     * segments: the length with which the rounds of units take least, a unit costing its tiles and two more. One
+     * row, 32,768 keys, 8 heads: 37 us with a round's worth of pieces, 58 with three rounds', 460 uncut; 16 rows x
+     * 2,048 keys x 32 heads on 8: 34 in two pieces, 41 in three (two rounds). A longer segment than the others is cut
+     * to the same pieces (single rows over 512, 77, 2,048 and 1 keys x 56 heads: 25 us, uncut 37), but where CTAs
+     * have many units anyway not finer than a CTA's share. Every piece writes its rows in F32 and they are read
+     * again: no more of that than there is to read of keys and values (1,000 rows, 16 heads on 2, 700 keys: 26 us in
+     * two parts, 19 in one). Two groups: two key tiles or more each. */
     const uint64_t worth = uint64_t(args.key_rows) * args.kv_heads / (uint64_t(args.query_rows) * args.heads * 2);
-    splits = splits > most ? most : splits;
-    splits = splits > worth ? worth : splits;
-    args.splits = splits < 1 ? 1 : uint32_t(splits);
-    units *= args.splits;
+    const uint64_t spread = (args.query_rows + per_item - 1) / per_item;
+    const uint64_t even_units = (spread > args.segment_count ? spread : args.segment_count) * args.head_units;
+    const uint64_t even_tiles = (tiles + args.segment_count - 1) / args.segment_count;
+    uint64_t piece = even_tiles, least = ~0ull;
+    for (uint64_t cuts = 1; cuts * GROUPS <= even_tiles; cuts++) {
+        const uint64_t rounds = (even_units * cuts + resident - 1) / resident, length = (even_tiles + cuts - 1) / cuts;
+        if (rounds * (GROUPS + 2) >= least) break;           /* no finer cut is faster */
+        if (rounds * (length + 2) < least) {
+            least = rounds * (length + 2);
+            piece = length;
+        }
+    }
+    const uint64_t share = even_units * even_tiles / resident;
+    if (piece < share) piece = share;
+    if (!worth || piece > tiles) piece = tiles;
+    if (worth && piece * worth < tiles) piece = (tiles + worth - 1) / worth;
+    const uint64_t pieces = (tiles + piece - 1) / piece;
+    args.per_piece = pieces > 1 ? uint32_t((1ull << 31) / piece) : 0;
+    /* most units there can be: every segment may end in a part of a tile, and have all key rows */
+    const uint64_t units = (args.query_rows / per_item + args.segment_count) * pieces * args.head_units;
     if (units > 0xffffffffull - 2 * resident) return h3b_fail(gpu, "cross attention has too many tiles");
     const unsigned grid = unsigned(units < resident ? units : resident);
     args.step_h = grid % args.head_units;
-    args.step_s = grid / args.head_units % args.splits;
-    args.step_i = grid / args.head_units / args.splits;
-    h3b_scratch scratch(gpu, args.splits > 1 ? size_t(args.splits) * args.query_rows * args.heads * (D + 2) * sizeof(float) : 0);
-    if (args.splits > 1) {
+    args.step_i = grid / args.head_units;
+    h3b_scratch scratch(gpu, pieces > 1 ? size_t(pieces) * args.query_rows * args.heads * (D + 2) * sizeof(float) : 0);
+    if (pieces > 1) {
         if (!scratch.data) return h3b_fail(gpu, "cross_sdpa_bf16: cannot allocate the partial results");
         args.partial_o = static_cast<float *>(scratch.data);
-        args.partial_ml = args.partial_o + size_t(args.splits) * args.query_rows * args.heads * D;
+        args.partial_ml = args.partial_o + size_t(pieces) * args.query_rows * args.heads * D;
     }
     h3b_cross_tc<D, GROUPS><<<grid, ct_threads<GROUPS>(), ct_smem<D, GROUPS>(), gpu->stream>>>(map_q, map_k, map_v, map_out, args);
-    if (args.splits > 1) {
+    if (pieces > 1) {
         const size_t warps = size_t(args.query_rows) * args.heads;
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3(unsigned((warps + 7) / 8));

@@ -131,6 +131,18 @@ def test_few_queries_over_long_states(gpu, dim, lengths):
     check(gpu, Case(segments, 4, 2, dim))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (8, 2, 64), (16, 2, 128)])
+@pytest.mark.parametrize("lengths", [
+    [(1, 100), (1, 4000), (1, 0), (2, 129), (1, 2047)], [(130, 1500), (1, 12000), (700, 10), (3, 0)], [(1, 20001)]])
+def test_segments_cut_into_different_numbers_of_pieces(gpu, heads, kv_heads, dim, lengths):
+    segments, q, k = [], 2, 1
+    for a, b in lengths:
+        segments.append([q, a, k, b])
+        q, k = q + a + 1, k + b + 3
+    case = Case(segments, heads, kv_heads, dim, query_rows=q + 1, key_rows=k + 130).spoil_gaps()
+    check(gpu, case, f"{lengths}")
+
+
 @pytest.mark.parametrize("dim", [8, 32, 40, 80, 96, 100, 256, 512, 1])
 def test_other_head_sizes(gpu, dim):
     check(gpu, Case([[0, 9, 0, 51], [9, 20, 60, 140]], 4, 2, dim).spoil_gaps(), f"dim {dim}")
