@@ -123,12 +123,14 @@ h3b_cross_simt(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t
  *   warp 0   TMA. Stage t % STAGES holds what the tensor core reads after the softmax of step t: V(t) and
  *            K(t + 1). With a unit's last step come the next unit's queries (one buffer per group: the
  *            scores of the last step have been computed by then).
- *   warp 1   tcgen05.mma, per step and group: O += P(t).V(t), then the group's scores Q.K(t + 1)^T. The tensor
- *            pipe does not drain between units: states are short (one to four steps), and a CTA per
+ *   warp 1   tcgen05.mma, per step and group: O += P(t).V(t), then the group's scores Q.K(t + 1)^T, at a unit's
+ *            end those of the next unit once its queries are there (the groups write their outputs meanwhile). The
+ *            tensor pipe does not drain between units: states are short (one to four steps), and a CTA per
  *            tile would spend half of its time filling and draining. All the group waits for collects on
- *            one barrier, go[group][t % 2]: the softmax warps' arrivals for P(t) and, for the first group, the
- *            bytes of V(t) and K(t + 1). Behind a unit's last P.V come the scores of the next unit, once its
- *            queries are there (the groups write their outputs meanwhile). The issuing warp is one instruction stream of 4 to 5 cycles an
+ *            two barriers: go[group][t % 2], the softmax warps' arrivals for the first half of P(t) and, for
+ *            the first group, the bytes of V(t) and K(t + 1); go2, the second half, whose exponentials are
+ *            computed while the first half is multiplied (1,664 rows x 257 keys x 24 heads 21.7 us, all of P
+ *            at once 22.0). The issuing warp is one instruction stream of 4 to 5 cycles an
  *            instruction: with a barrier each for P, K, V and Q it needed 3,270 cycles per step of two
  *            groups without a single MMA. P (BF16) overwrites the scores it came from and is the A
  *            operand of P.V; the in-order pipe keeps the next scores behind it.
@@ -300,7 +302,8 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     const uint32_t first = bars;                                    /* K(0)                  */
     const uint32_t queries = first + 8;                             /* a unit's query tiles  */
     const uint32_t go = queries + 8;                                /* [group][step % 2] = 4 */
-    const uint32_t s_full = go + 32;                                /* [group] = 2: scores   */
+    const uint32_t go2 = go + 32;                                   /* [group][step % 2]: P complete */
+    const uint32_t s_full = go2 + 32;                               /* [group] = 2: scores   */
     const uint32_t o_done = s_full + 16;                            /* [group] = 2           */
     const uint32_t seen = o_done + 16;                              /* [step % 2]: scores of all groups seen complete */
     const uint32_t tail = seen + 16;                                /* [step % 2]: V tile that has to be cleared in part */
@@ -318,7 +321,10 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         *stop = 0;
         mbar_init(first, 1);
         mbar_init(queries, 1);
-        for (int i = 0; i < 2 * GROUPS; i++) mbar_init(go + 8 * i, i < 2 ? 9 : 8);      /* 8 softmax warps, the producer */
+        for (int i = 0; i < 2 * GROUPS; i++) {
+            mbar_init(go + 8 * i, i < 2 ? 9 : 8);      /* 8 softmax warps, the producer */
+            mbar_init(go2 + 8 * i, 8);
+        }
         for (int i = 0; i < 2; i++) { mbar_init(seen + 8 * i, 1); mbar_init(tail + 8 * i, 1); }
         for (int g = 0; g < GROUPS; g++) {
             mbar_init(s_full + 8 * g, 1);
@@ -450,7 +456,7 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         auto step = [&](auto parity_const) {
             constexpr int PARITY = decltype(parity_const)::value;
             constexpr integral_constant<int, PARITY % STAGES> stage{};
-            const bool last = left == 1;
+            const bool last = left == 1, more = !last || n_steps;
             auto group = [&](auto g_const) {
                 constexpr int g = decltype(g_const)::value;
                 if (!__all_sync(0xffffffffu, ready != 0u) && !wait(go + 16 * g + 8 * PARITY, phase)) return false;
@@ -458,14 +464,30 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 const uint32_t d = tmem_base + COL_O + g * D, a = tmem_base + g * CT, v_lo = v_lo0 + stage.value * STAGE;
                 if (start) umma_ts<false>(d, a, v_lo, idesc_pv, leader);
                 else umma_ts<true>(d, a, v_lo, idesc_pv, leader);
-#pragma unroll
-                for (uint32_t kk = 1; kk < 8; kk++)       /* P of keys 64.. lies on the columns of their scores */
-                    umma_ts<true>(d, a + (kk >> 2) * 64 + (kk & 3) * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader);
-                if (last) umma_commit_if(o_done + 8 * g, leader);
-                else issue_qk(g_const, stage, zero, most);
+                /* P of keys 64.. lies on the columns of their scores; first the halves' first 32 keys */
+                auto pv = [&](uint32_t kk) { umma_ts<true>(d, a + (kk >> 2) * 64 + (kk & 3) * 8, v_lo + kk * (2048 >> 4), idesc_pv, leader); };
+                pv(1);
+                pv(4);
+                const uint32_t complete = mbar_test(go2 + 16 * g + 8 * PARITY, phase);
+                pv(5);
+                if (!__all_sync(0xffffffffu, complete != 0u) && !wait(go2 + 16 * g + 8 * PARITY, phase)) return false;
+                tc_fence_after();
+                pv(2);
+                pv(3);
+                pv(6);
+                pv(7);
+                if (last) {
+                    umma_commit_if(o_done + 8 * g, leader);
+                    if (g == 0 && more) {                 /* the next unit's queries */
+                        if (!wait(queries, q_phase)) return false;
+                        q_phase ^= 1;
+                        tc_fence_after();
+                    }
+                }
+                if (more) issue_qk(g_const, stage, zero, most);
                 if (g + 1 < GROUPS) ready = mbar_test(go + 16 + 8 * PARITY, phase);
                 else ready = mbar_test(go + 8 * (PARITY ^ 1), phase ^ PARITY);
-                if (!last) issue_qk(g_const, stage, most, all);
+                if (more) issue_qk(g_const, stage, most, all);
                 return true;
             };
             if (!group(integral_constant<int, 0>{})) return false;
@@ -475,14 +497,7 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             left--;
             if (last) {
                 left = n_steps;
-                if (left) {
-                    if (!wait(queries, q_phase)) return false;
-                    q_phase ^= 1;
-                    tc_fence_after();
-                    issue_qk(zero, stage, zero, all);
-                    if constexpr (GROUPS == 2) issue_qk(integral_constant<int, 1>{}, stage, zero, all);
-                    n_steps = next_unit();
-                }
+                if (left) n_steps = next_unit();
             }
             return left != 0;
         };
@@ -588,14 +603,6 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 const float neg_m = reference == -INFINITY ? 0.0f : -reference;
                 const uint64_t neg_m2 = pack_f32x2(neg_m, neg_m);
                 uint64_t sum_a = 0, sum_b = 0;
-                /* P of 32 keys lands on columns in front of the scores that are still to be read */
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t packed[16];
-                    if (c) scores(c);
-                    ct_exponentials(s, scale2, neg_m2, packed, sum_a, sum_b);
-                    ct_st16(tmem_s + c * 16, packed);
-                }
                 if (u.dirty && j + 1 == steps && g == 0) {
                     /* value rows that are not the segment's: cleared before anybody's P.V, which is issued
                      * behind this group's arrival */
@@ -609,10 +616,24 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                     fence_async_smem();
                     tail_phase ^= 1u << (t & 1u);
                 }
+                /* P of 32 keys lands on columns in front of the scores that are still to be read */
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t packed[16];
+                    if (c) scores(c);
+                    ct_exponentials(s, scale2, neg_m2, packed, sum_a, sum_b);
+                    ct_st16(tmem_s + c * 16, packed);
+                    if (c == 0) {
+                        tmem_st_wait_all();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(go + 16 * g + 8 * (t & 1u));
+                    }
+                }
                 tmem_st_wait_all();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(go + 16 * g + 8 * (t & 1u));
+                if (lane == 0) mbar_arrive(go2 + 16 * g + 8 * (t & 1u));
                 float s0, s1, s2, s3;
                 unpack_f32x2(sum_a, s0, s1);
                 unpack_f32x2(sum_b, s2, s3);
