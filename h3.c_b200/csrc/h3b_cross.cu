@@ -953,11 +953,14 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
         args.head_units = heads / args.pack;
         args.units_per_kv = group / args.pack;
         args.scale_log2 = scale * 1.4426950408889634f;
-        /* One group per CTA, two CTAs per SM: where segments hold a tile of rows or less on average, and where
-         * units of two tiles would leave more than half of the SMs idle (300 rows x 32 heads on 8, 300 keys,
-         * head_dim 64: 10.6 against 12.4 us; 1,664 x 24 heads x 257 keys, which fills them: 22.8 against 22.6). */
+        /* One group per CTA, two CTAs per SM: where segments hold a tile of rows or less on average, and where units of two
+         * tiles would leave more than half of the SMs idle (900 rows x 24 heads x 300 keys, 96 such units: two
+         * groups 13.9 us, one 16.0); with head_dim 64, where loads and products are half as long, up to two rounds of
+         * them (1,797 rows x 32 heads on 8 x 77 keys, 232 units: 12.0, one group 11.0; 6,400 rows x 56 heads x 77
+         * keys, 1,456 units: 33.4, 41.2). */
         const uint64_t tile_rows = CT >> args.pack_log2, pairs = (query_rows / (2 * tile_rows) + segment_count) * args.head_units;
-        const bool few = query_rows <= segment_count * tile_rows || 2 * pairs <= uint64_t(gpu->sm_count);
+        const uint64_t sms = uint64_t(gpu->sm_count);
+        const bool few = query_rows <= segment_count * tile_rows || (head_dim == 64 ? pairs <= 2 * sms : 2 * pairs <= sms);
         if (few) return head_dim == 128 ? ct_launch<128, 1>(gpu, args, q, k, v) : ct_launch<64, 1>(gpu, args, q, k, v);
         return head_dim == 128 ? ct_launch<128, 2>(gpu, args, q, k, v) : ct_launch<64, 2>(gpu, args, q, k, v);
     }
