@@ -99,6 +99,7 @@ constexpr int LR_M = 128;                    /* rows of an instruction: x rows (
 constexpr int LR_K = 64;                     /* one 128-byte swizzle line */
 constexpr int LR_A_BYTES = LR_M * LR_K * 2;
 constexpr int LR_THREADS = 192;              /* TMA, MMA, 4 epilogue warps */
+constexpr uint32_t LR_SPLIT = 8;             /* CTAs of a cluster, at most */
 constexpr int LR_STAGES = 8;                 /* barriers laid out; a launch uses `stages` of them */
 constexpr int LR_BAR_BYTES = 256;
 constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1024;
@@ -180,15 +181,34 @@ __device__ __forceinline__ uint32_t adapter_of(const h3b_lora_task &task, uint32
     const uint32_t a = row >= task.rows ? kNone : task.row_adapter ? __ldg(task.row_adapter + row) : 0;
     return a < task.adapters ? a : kNone;
 }
+/* A thread's rows of the tile, threadIdx.x and the one blockDim.x on: with 192 threads or more two loads cover any
+ * tile. Asked for first of all and used behind the set-up: one after the other, the row's adapter, the tile's
+ * second rows and the scale cost three memory latencies (3.5 us of a kernel of 13 us). */
+struct TileRows {
+    uint32_t a[2], rows;        /* rows: how many of the two exist */
+};
+__device__ __forceinline__ TileRows load_rows(const h3b_lora_task &task, uint32_t tile) {
+    TileRows r = {{kNone, kNone}, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 2; i++) {
+        const uint32_t at = threadIdx.x + i * blockDim.x;
+        if (at < task.tile_rows && tile * task.tile_rows + at < task.rows) {
+            r.a[i] = adapter_of(task, tile * task.tile_rows + at);
+            r.rows = i + 1;
+        }
+    }
+    return r;
+}
 /* all threads; returns the number of entries */
-__device__ __forceinline__ uint32_t find_entries(Entries &s, const h3b_lora_task &task, uint32_t tile) {
+__device__ __forceinline__ uint32_t find_entries(Entries &s, const TileRows &rows) {
     const uint32_t lane = threadIdx.x & 31;
     if (threadIdx.x < kMaxAdapters / 32) s.present[threadIdx.x] = 0;
     if (threadIdx.x == 0) s.without = 0;
     __syncthreads();
-    for (uint32_t r = threadIdx.x; r < task.tile_rows && tile * task.tile_rows + r < task.rows; r += blockDim.x) {
-        const uint32_t a = adapter_of(task, tile * task.tile_rows + r);
-        if (a != kNone) atomicOr(&s.present[a >> 5], 1u << (a & 31));
+#pragma unroll
+    for (uint32_t i = 0; i < 2; i++) {
+        if (i >= rows.rows) break;
+        if (rows.a[i] != kNone) atomicOr(&s.present[rows.a[i] >> 5], 1u << (rows.a[i] & 31));
         else s.without = 1;
     }
     __syncthreads();
@@ -235,20 +255,20 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = gridDim.x, part = blockIdx.x, row0 = blockIdx.y * LR_M, tile = row0 / task.tile_rows;
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
+    const TileRows rows = load_rows(task, tile);
+    const uint32_t own_a = threadIdx.x < LR_M ? adapter_of(task, row0 + threadIdx.x) : kNone;
+    if (threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_down) : "memory");
     Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 2, true);
+    const float own_s = own_a != kNone && task.scale ? __ldg(task.scale + own_a) : 1.0f;
     const uint32_t early = blockIdx.z == 0 ? min(args.ring.stages, kb1 - kb0) : 0;
     if (threadIdx.x == 0)
         for (uint32_t i = 0; i < early; i++) {
             mbar_expect_tx(ring.full + 8 * i, LR_A_BYTES);
             tma_load_2d(ring.stage0 + i * args.ring.stage_bytes, &map_x, ring.full + 8 * i, int((kb0 + i) * LR_K), int(row0));
         }
-    const uint32_t count = find_entries(found, task, tile);
+    const uint32_t count = find_entries(found, rows);
     if (blockIdx.z == 0 && part == 0 && row0 == tile * task.tile_rows) publish_entries(found, task, tile, count);
-    if (threadIdx.x < LR_M) {
-        const uint32_t a = adapter_of(task, row0 + threadIdx.x);
-        own[threadIdx.x] = entry_of(found, a);
-        own_scale[threadIdx.x] = a != kNone && task.scale ? task.scale[a] : 1.0f;
-    }
+    if (threadIdx.x < LR_M) own[threadIdx.x] = entry_of(found, own_a);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -322,6 +342,7 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 tc_fence_before();
             }
         }
+        if (threadIdx.x < LR_M) own_scale[threadIdx.x] = own_s;
         __syncwarp();
         cluster_sync_all();
         if (!*ring.stop) {
@@ -336,12 +357,15 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 if (own[r] == e) {
                     const uint32_t c = (e - e0) * args.rank16 + j;
                     const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4) * 4;
-                    for (uint32_t p = 0; p < split; p++) {
-                        float4 x;
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_map(at, p)) : "memory");
-                        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-                    }
+                    float4 x[LR_SPLIT];
+#pragma unroll
+                    for (uint32_t p = 0; p < LR_SPLIT; p++)
+                        if (p < split)
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(x[p].x), "=f"(x[p].y), "=f"(x[p].z), "=f"(x[p].w) : "r"(cluster_map(at, p)) : "memory");
+#pragma unroll
+                    for (uint32_t p = 0; p < LR_SPLIT; p++)
+                        if (p < split) { v.x += x[p].x; v.y += x[p].y; v.z += x[p].z; v.w += x[p].w; }
                     const float s = own_scale[r];
                     v.x = j < task.rank ? v.x * s : 0.0f;
                     v.y = j + 1 < task.rank ? v.y * s : 0.0f;
@@ -372,25 +396,26 @@ h3b_lora_down_few(const __grid_constant__ h3b_lora_task task) {
     h3b_let_next_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t row = blockIdx.x, j = blockIdx.y * LF_SUMS + warp / 4, a = adapter_of(task, row);
+    const TileRows rows = load_rows(task, 0);
+    const float s = a != kNone && task.scale ? __ldg(task.scale + a) : 1.0f;
     float sum = 0.0f;
     if (a != kNone && j < task.rank) {
         const uint4 *x = reinterpret_cast<const uint4 *>(task.x + size_t(row) * task.k);
         const uint4 *d = reinterpret_cast<const uint4 *>(task.down + (size_t(a) * task.rank + j) * task.k);
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
         for (uint32_t i = (warp & 3) * 32 + lane; i < task.k / 8; i += 128) {
             const uint4 u = __ldg(x + i), v = __ldg(d + i);
             const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int q = 0; q < 4; q++) s[q] = fmaf(h3b_hi(us[q]), h3b_hi(vs[q]), fmaf(h3b_lo(us[q]), h3b_lo(vs[q]), s[q]));
+            for (int q = 0; q < 4; q++) sums[q] = fmaf(h3b_hi(us[q]), h3b_hi(vs[q]), fmaf(h3b_lo(us[q]), h3b_lo(vs[q]), sums[q]));
         }
-        sum = h3b_warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+        sum = h3b_warp_sum((sums[0] + sums[1]) + (sums[2] + sums[3]));
     }
     if (lane == 0) part[warp] = sum;
-    const uint32_t count = find_entries(found, task, 0);          /* has block barriers */
+    const uint32_t count = find_entries(found, rows);          /* has block barriers */
     if (blockIdx.x == 0 && blockIdx.y == 0) publish_entries(found, task, 0, count);
     const uint32_t mine = entry_of(found, a);
-    const float s = a != kNone && task.scale ? task.scale[a] : 1.0f;
     for (uint32_t i = threadIdx.x; i < count * LF_SUMS; i += 32 * LF_WARPS) {
         const uint32_t e = i / LF_SUMS, q = i % LF_SUMS, jj = blockIdx.y * LF_SUMS + q;
         const float v = ((part[4 * q] + part[4 * q + 1]) + (part[4 * q + 2] + part[4 * q + 3])) * s;
@@ -530,13 +555,14 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             for (uint32_t r = part + split * (threadIdx.x >> 6); r < live; r += 2 * split) {
                 const uint32_t at = ring.stage0 + (r * LR_M + 2 * (threadIdx.x & 63)) * 4;
                 float v0 = 0.0f, v1 = 0.0f;
-                for (uint32_t p = 0; p < split; p++) {
-                    const uint32_t from = cluster_map(at, p);
-                    float x0, x1;
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x0), "=f"(x1) : "r"(from) : "memory");
-                    v0 += x0;
-                    v1 += x1;
-                }
+                float x0[LR_SPLIT], x1[LR_SPLIT];
+#pragma unroll
+                for (uint32_t p = 0; p < LR_SPLIT; p++)      /* all on the way before the first is used */
+                    if (p < split)
+                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x0[p]), "=f"(x1[p]) : "r"(cluster_map(at, p)) : "memory");
+#pragma unroll
+                for (uint32_t p = 0; p < LR_SPLIT; p++)
+                    if (p < split) { v0 += x0[p]; v1 += x1[p]; }
                 v0 += b0;
                 v1 += b1;
                 if (mixed && (h3b_not_finite(v0) || h3b_not_finite(v1))) {
@@ -675,7 +701,7 @@ uint64_t resident_clusters(int device, Kernel *kernel, uint32_t split, size_t sm
  * CTAs per SM: 21.6 us in 3 parts, 18.5 in 4, 16.8 in 5, 15.9 in 6, 26.3 in 7 (a second round). */
 template <class Kernel>
 uint32_t split_for(h3_gpu *gpu, Kernel *kernel, size_t smem, uint32_t per_sm, uint64_t tiles, uint32_t k_blocks) {
-    for (uint32_t split = 8; split > 1; split--)
+    for (uint32_t split = LR_SPLIT; split > 1; split--)
         if (split * 4 <= k_blocks && tiles <= per_sm * resident_clusters(gpu->device, kernel, split, smem)) return split;
     return 1;
 }
@@ -697,9 +723,11 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool beh
     down.ring.wait_cycles = gpu->wait_cycles;
     down.ring.stage_bytes = LR_A_BYTES + columns * LR_K * 2;
     down.ring.tmem_columns = tmem_columns_for(columns);
-    /* two CTAs per SM where there are as many and the joined accumulators (128 x columns F32) leave room for
-     * it; else deeper rings, since a CTA's stream is its bytes in flight over the memory's latency */
-    const bool two = columns <= 128 && uint64_t(row_blocks) * 8 > uint64_t(gpu->sm_count);
+    /* Two CTAs per SM where they would fill more than half of the SMs alone and the joined accumulators (128 x columns F32)
+     * leave room for it, so that the projection can begin on the others (1,664 rows, 7,168 -> 5,376, rank 64, 104
+     * CTAs: 122 us, one per SM 127); else deeper rings, since a CTA's stream is its bytes in flight over the memory's
+     * latency (800 rows, 14,336 -> 5,376, rank 128, 56 CTAs: 138 us, two per SM 139.3). */
+    const bool two = columns <= 128 && uint64_t(row_blocks) * 2 * LR_SPLIT > uint64_t(gpu->sm_count);
     const uint32_t want = two ? 106 << 10 : 200 << 10;
     down.ring.stages = want / down.ring.stage_bytes;
     if (down.ring.stages > uint32_t(LR_STAGES)) down.ring.stages = LR_STAGES;
