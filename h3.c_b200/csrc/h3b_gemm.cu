@@ -467,8 +467,13 @@ __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_
                                                        __uint_as_float(r[2 * i + 1]));
                         }
                         if constexpr (EPI == H3B_EPI_LORA) {
-                            if (mixed) {
-                                /* not finite: maybe another row's adapter (see h3b_lora_element) */
+                            /* Something not finite (times zero: NaN, found once for 32 columns): maybe another row's
+                             * adapter (see h3b_lora_element). A test and branch per pair cost 1,003 rows x 5,376
+                             * columns 6 us. */
+                            float zero = 0.0f;
+    #pragma unroll
+                            for (int i = 0; i < 32; i++) zero = fmaf(__uint_as_float(r[i]), 0.0f, zero);
+                            if (mixed && zero != 0.0f) {
     #pragma unroll
                                 for (int i = 0; i < 16; i++) {
                                     float lo = __uint_as_float(r[2 * i]), hi = __uint_as_float(r[2 * i + 1]);
