@@ -156,18 +156,18 @@ __device__ __forceinline__ uint32_t ring_tmem(const Ring &r) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(r.holder));
     return tmem;
 }
-__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r, uint32_t tmem) {
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    if (*r.stop) {
-        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_GEMM_TIMEOUT));
-        for (int i = 0; i < 1000; i++) __nanosleep(1000);
-        __syncthreads();
-    }
+__device__ __forceinline__ void ring_free(const RingArgs &args, uint32_t tmem) {
     if (threadIdx.x >> 5 == 1) {
         tc_fence_after();
         tmem_free(tmem, args.tmem_columns);
+    }
+    __syncwarp();
+}
+/* a wait that ran out: the status, and time for copies that may be in flight to land */
+__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r) {
+    if (*r.stop) {
+        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_GEMM_TIMEOUT));
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
     }
 }
 
@@ -382,7 +382,11 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         cluster_sync_all();
         tc_fence_after();
     }
-    ring_close(args.ring, ring, tmem);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    ring_free(args.ring, tmem);
+    ring_close(args.ring, ring);
     h3b_wait_for_launch();               /* the padded up rows, where a launch in front writes them: done before this one is */
 }
 
@@ -448,8 +452,12 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
     const uint32_t b_bytes = task.tile_rows * LR_K * 2;
     Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1, false);
-    __shared__ uint32_t entries;
+    __shared__ uint32_t entries, rows_differ;
     __shared__ uint16_t adapter[LR_M];
+    /* the join's threads (the epilogue's warps) have two weight rows of every second of their CTA's x rows */
+    const uint32_t col = w0 + 2 * (threadIdx.x & 63);
+    uint32_t bias = 0;
+    if (warp >= 2 && task.bias && col < task.n) bias = __ldg(reinterpret_cast<const uint32_t *>(task.bias + col));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -514,9 +522,12 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         if (warp == 2) {
             /* what the launch in front found */
             h3b_wait_for_launch();
-            const uint32_t count = task.counts[tile] & ~H3B_LORA_MIXED;
+            const uint32_t found = task.counts[tile], count = found & ~H3B_LORA_MIXED;
             for (uint32_t e = lane; e < count; e += 32) adapter[e] = uint16_t(task.entries[size_t(tile) * task.max_entries + e]);
-            if (lane == 0) entries = count;
+            if (lane == 0) {
+                entries = count;
+                rows_differ = found & H3B_LORA_MIXED;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(ring.info);
         }
@@ -539,21 +550,19 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             }
         }
     }
+    /* tensor memory goes back while the cluster meets */
     __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    ring_free(args.ring, tmem);
     cluster_sync_all();
-    if (!*ring.stop && threadIdx.x < LR_M) {
-        /* rows part, part + split, ...; a thread has two weight rows of every second of them */
-        h3b_wait_for_launch();
-        const bool mixed = task.counts[tile] & H3B_LORA_MIXED;
-        const uint32_t col = w0 + 2 * (threadIdx.x & 63);
+    if (!*ring.stop && warp >= 2) {
+        /* rows part, part + split, ... */
+        h3b_wait_for_launch();               /* the recomputed elements read what the launch in front wrote */
+        const bool mixed = rows_differ;
         if (col < task.n) {
-            float b0 = 0.0f, b1 = 0.0f;
-            if (task.bias) {
-                const uint32_t b = *reinterpret_cast<const uint32_t *>(task.bias + col);
-                b0 = h3b_lo(b);
-                b1 = h3b_hi(b);
-            }
-            for (uint32_t r = part + split * (threadIdx.x >> 6); r < live; r += 2 * split) {
+            const float b0 = h3b_lo(bias), b1 = h3b_hi(bias);
+            for (uint32_t r = part + split * ((threadIdx.x >> 6) - 1); r < live; r += 2 * split) {
                 const uint32_t at = ring.stage0 + (r * LR_M + 2 * (threadIdx.x & 63)) * 4;
                 float v0 = 0.0f, v1 = 0.0f;
                 float x0[LR_SPLIT], x1[LR_SPLIT];
@@ -574,8 +583,9 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             }
         }
     }
-    cluster_sync_all();
-    ring_close(args.ring, ring, tmem);
+    __syncwarp();
+    cluster_sync_all();      /* nobody leaves while its shared memory may be read */
+    ring_close(args.ring, ring);
 }
 
 /* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes. 8 elements a thread. */
