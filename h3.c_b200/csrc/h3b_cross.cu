@@ -28,6 +28,8 @@ struct Segment {
 __device__ __forceinline__ Segment load_segment(const uint32_t *segments, uint32_t index, uint32_t query_rows,
                                                 uint32_t key_rows) {
     if (!segments) return {0u, query_rows, 0u, key_rows};
+    /* Read-only loads (plain ones cost single rows 0.5 us of 25): behind griddepcontrol.wait what is in front of the call
+     * has ended, and nothing of this launch has touched the table before. */
     const uint4 raw = make_uint4(__ldg(segments + 4 * index), __ldg(segments + 4 * index + 1),
                                  __ldg(segments + 4 * index + 2), __ldg(segments + 4 * index + 3));
     Segment s;
@@ -318,7 +320,6 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     volatile float *xchg = reinterpret_cast<volatile float *>(ct_smem_raw + (bars - base) + CT_BARS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long budget = args.wait_cycles;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      /* the merge, which waits for this launch's end */
     if ((base & 1023u) != 0) {       /* swizzled tiles need 1024-byte alignment */
         if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_ATTN_TIMEOUT));
         return;
@@ -342,6 +343,10 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_out) : "memory");
     }
+    /* The launch in front of this one has ended. Tensor memory is taken behind that, so that nothing in front can wait for
+     * it; the merge, which waits for this one's end, may begin. */
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) tmem_alloc(holder, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
@@ -884,19 +889,26 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
         args.partial_o = static_cast<float *>(scratch.data);
         args.partial_ml = args.partial_o + size_t(pieces) * args.query_rows * args.heads * D;
     }
-    h3b_cross_tc<D, GROUPS><<<grid, ct_threads<GROUPS>(), ct_smem<D, GROUPS>(), gpu->stream>>>(map_q, map_k, map_v, map_out, args);
+    /* Both launches may begin while what is in front of them ends, and wait inside: their set-up comes out of
+     * its time. Not the first one while capturing, where an allocation is in front of it. */
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(ct_threads<GROUPS>());
+    config.dynamicSmemBytes = ct_smem<D, GROUPS>();
+    config.stream = gpu->stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = scratch.captured ? 0 : 1;
+    cudaLaunchKernelEx(&config, h3b_cross_tc<D, GROUPS>, map_q, map_k, map_v, map_out, args);      /* an error is reported by h3b_launched */
     if (pieces > 1) {
         const size_t warps = size_t(args.query_rows) * args.heads;
-        cudaLaunchConfig_t config = {};
         config.gridDim = dim3(unsigned((warps + 7) / 8));
         config.blockDim = dim3(256);
-        config.stream = gpu->stream;
-        cudaLaunchAttribute attribute;
-        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attribute.val.programmaticStreamSerializationAllowed = 1;
-        config.attrs = &attribute;
+        config.dynamicSmemBytes = 0;
         config.numAttrs = 1;
-        cudaLaunchKernelEx(&config, h3b_cross_merge<D>, args);      /* an error is reported by h3b_launched */
+        cudaLaunchKernelEx(&config, h3b_cross_merge<D>, args);
     }
     return h3b_launched(gpu, "cross_sdpa_bf16", H3B_SDPA);
 }

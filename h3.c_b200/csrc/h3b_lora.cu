@@ -122,10 +122,8 @@ struct Ring {
     uint32_t stage0, full, empty, done, info, holder;
     volatile int *stop;
 };
-/* addresses, and (thread 0) the barriers: `arrivals` per full barrier. `let_next`: the launch behind this one, which may
- * begin early, does so when every CTA has its tensor memory: none can wait for columns of a CTA that waits
- * for this launch. */
-__device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, int *stop_flag, uint32_t arrivals, bool let_next) {
+/* addresses, and (thread 0) the barriers: `arrivals` per full barrier */
+__device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, int *stop_flag, uint32_t arrivals) {
     Ring r;
     r.stage0 = (smem_u32(raw) + 1023u) & ~1023u;
     r.full = r.stage0 + args.stages * args.stage_bytes;
@@ -144,10 +142,7 @@ __device__ __forceinline__ Ring ring_begin(const RingArgs &args, uint8_t *raw, i
         mbar_init(r.info, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (threadIdx.x >> 5 == 1) {
-        tmem_alloc(r.holder, args.tmem_columns);
-        if (let_next) h3b_let_next_launch();
-    }
+    if (threadIdx.x >> 5 == 1) tmem_alloc(r.holder, args.tmem_columns);
     return r;
 }
 /* behind the block barrier that follows ring_begin: the accumulator's address */
@@ -179,7 +174,7 @@ struct Entries {
 };
 constexpr uint32_t kNone = 0xffffffffu;
 __device__ __forceinline__ uint32_t adapter_of(const h3b_lora_task &task, uint32_t row) {
-    const uint32_t a = row >= task.rows ? kNone : task.row_adapter ? __ldg(task.row_adapter + row) : 0;
+    const uint32_t a = row >= task.rows ? kNone : task.row_adapter ? task.row_adapter[row] : 0;
     return a < task.adapters ? a : kNone;
 }
 /* A thread's rows of the tile, threadIdx.x and the one blockDim.x on: with 192 threads or more two loads cover any
@@ -256,11 +251,15 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = gridDim.x, part = blockIdx.x, row0 = blockIdx.y * LR_M, tile = row0 / task.tile_rows;
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
+    if (threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_down) : "memory");
+    /* Tensor memory behind the wait for what is in front, and the launch behind let go behind that: nobody ever waits for
+     * columns of a CTA that waits for it. */
+    if (task.first) h3b_wait_for_launch();
+    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 2);
+    if (warp == 1) h3b_let_next_launch();
     const TileRows rows = load_rows(task, tile);
     const uint32_t own_a = threadIdx.x < LR_M ? adapter_of(task, row0 + threadIdx.x) : kNone;
-    if (threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_down) : "memory");
-    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 2, true);
-    const float own_s = own_a != kNone && task.scale ? __ldg(task.scale + own_a) : 1.0f;
+    const float own_s = own_a != kNone && task.scale ? task.scale[own_a] : 1.0f;
     const uint32_t early = blockIdx.z == 0 ? min(args.ring.stages, kb1 - kb0) : 0;
     if (threadIdx.x == 0)
         for (uint32_t i = 0; i < early; i++) {
@@ -398,11 +397,12 @@ __global__ void __launch_bounds__(32 * LF_WARPS)
 h3b_lora_down_few(const __grid_constant__ h3b_lora_task task) {
     __shared__ Entries found;
     __shared__ float part[LF_WARPS];
+    if (task.first) h3b_wait_for_launch();
     h3b_let_next_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t row = blockIdx.x, j = blockIdx.y * LF_SUMS + warp / 4, a = adapter_of(task, row);
     const TileRows rows = load_rows(task, 0);
-    const float s = a != kNone && task.scale ? __ldg(task.scale + a) : 1.0f;
+    const float s = a != kNone && task.scale ? task.scale[a] : 1.0f;
     float sum = 0.0f;
     if (a != kNone && j < task.rank) {
         const uint4 *x = reinterpret_cast<const uint4 *>(task.x + size_t(row) * task.k);
@@ -410,7 +410,7 @@ h3b_lora_down_few(const __grid_constant__ h3b_lora_task task) {
         float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
         for (uint32_t i = (warp & 3) * 32 + lane; i < task.k / 8; i += 128) {
-            const uint4 u = __ldg(x + i), v = __ldg(d + i);
+            const uint4 u = x[i], v = d[i];
             const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int q = 0; q < 4; q++) sums[q] = fmaf(h3b_hi(us[q]), h3b_hi(vs[q]), fmaf(h3b_lo(us[q]), h3b_lo(vs[q]), sums[q]));
@@ -451,13 +451,13 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const uint32_t row0 = tile * task.tile_rows, live = min(task.tile_rows, task.rows - row0);
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
     const uint32_t b_bytes = task.tile_rows * LR_K * 2;
-    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1, false);
+    Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1);
     __shared__ uint32_t entries, rows_differ;
     __shared__ uint16_t adapter[LR_M];
     /* the join's threads (the epilogue's warps) have two weight rows of every second of their CTA's x rows */
     const uint32_t col = w0 + 2 * (threadIdx.x & 63);
     uint32_t bias = 0;
-    if (warp >= 2 && task.bias && col < task.n) bias = __ldg(reinterpret_cast<const uint32_t *>(task.bias + col));
+    if (warp >= 2 && task.bias && col < task.n) bias = *reinterpret_cast<const uint32_t *>(task.bias + col);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -591,6 +591,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 /* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes. 8 elements a thread. */
 __global__ void __launch_bounds__(256)
 h3b_lora_pad_up(const uint16_t *__restrict__ up, uint16_t *up8, size_t rows, uint32_t rank, uint32_t rank8) {
+    h3b_wait_for_launch();
     h3b_let_next_launch();
     const uint32_t pieces = rank8 / 8;
     const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -717,9 +718,11 @@ uint32_t split_for(h3_gpu *gpu, Kernel *kernel, size_t smem, uint32_t per_sm, ui
     return 1;
 }
 
-/* Rows [0, task.rows) on the tensor cores; scratch as laid out by the caller. `behind`: the launch that pads up is
- * in front on the stream. */
-int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool behind, bool captured) {
+/* Rows [0, task.rows) on the tensor cores; scratch as laid out by the caller. The first launch of a call may begin while
+ * the one in front of the call ends and waits inside; not while capturing, where the node in front is the
+ * scratch's allocation. */
+int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool captured) {
+    const bool dependent = !captured || !task.first;
     const uint32_t k_blocks = (task.k + LR_K - 1) / LR_K;
     const uint32_t tiles = (task.rows + task.tile_rows - 1) / task.tile_rows, row_blocks = (task.rows + LR_M - 1) / LR_M;
     CUtensorMap map_x, map_down;
@@ -753,9 +756,9 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool beh
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
     /* by warps while that reads the inputs a few times at most from L2 */
     if (few && task.rows <= uint32_t(LR_M) && uint64_t(task.rows) * task.rank <= 2048)
-        launch_cluster(gpu, h3b_lora_down_few, dim3(task.rows, task.rank8 / LF_SUMS), 32 * LF_WARPS, 1, 0, behind, task);
+        launch_cluster(gpu, h3b_lora_down_few, dim3(task.rows, task.rank8 / LF_SUMS), 32 * LF_WARPS, 1, 0, dependent, task);
     else
-        launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, side), LR_THREADS, down_split, ring_smem(down.ring), behind,
+        launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, side), LR_THREADS, down_split, ring_smem(down.ring), dependent,
                        map_x, map_down, down);
     if (cudaGetLastError() != cudaSuccess) return h3b_fail(gpu, "linear_lora_bf16: the low-rank rows cannot be launched");
     if (!few) {
@@ -860,7 +863,8 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
         if (up_bytes) {
             uint16_t *up8 = reinterpret_cast<uint16_t *>(at + t_bytes);
             const size_t up_rows = size_t(adapters) * output_dim;
-            h3b_lora_pad_up<<<unsigned((up_rows * (task.rank8 / 8) + 255) / 256), 256, 0, gpu->stream>>>(u, up8, up_rows, rank, task.rank8);
+            launch_cluster(gpu, h3b_lora_pad_up, dim3(unsigned((up_rows * (task.rank8 / 8) + 255) / 256)), 256, 1, 0, !scratch.captured, u, up8,
+                           up_rows, rank, task.rank8);
             task.up8 = up8;
         }
         for (size_t tile = 0; tile < all_tiles; tile += chunk_tiles) {
@@ -870,7 +874,8 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
             part.x = x + row0 * input_dim;
             part.out = y + row0 * output_dim;
             part.row_adapter = map ? map + row0 : nullptr;
-            if (!lora_tensor_cores(gpu, part, few, up_bytes && !tile, scratch.captured)) return 0;
+            part.first = !up_bytes || tile;
+            if (!lora_tensor_cores(gpu, part, few, scratch.captured)) return 0;
         }
         return h3b_launched(gpu, "linear_lora_bf16", kind);
     }

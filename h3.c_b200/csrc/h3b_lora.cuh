@@ -19,6 +19,7 @@ struct h3b_lora_task {
     uint16_t *out;
     uint32_t rows, k, n, adapters, rank, rank8;
     uint32_t tile_rows, max_entries;
+    uint32_t first;                 /* the low-rank rows are the call's first launch: it waits for what is in front of the call */
     uint32_t *counts;               /* [tile]: entries, bit 31: rows of the tile differ in their adapter */
     uint32_t *entries;              /* [tile][max_entries]: adapter of the entry */
     uint16_t *t;                    /* [tile][max_entries][tile_rows][rank8] */

@@ -102,3 +102,48 @@ def test_conditioning_without_requests_adds_nothing(pkg):
         assert np.array_equal(out.read(), heads)
     finally:
         gpu.close()
+
+
+@pytest.mark.parametrize("rows,rank", [(1, 16), (70, 12), (640, 16)])
+def test_a_chain_of_calls_equals_the_calls_one_by_one(pkg, rows, rank):
+    """Every call reads what the one in front of it wrote (their launches may begin before it has ended), the table
+    and the row map included: the same bits as with the stream drained in between."""
+    heads, adapters, states, steps = 8, 3, 700, 12
+    width = heads * 128
+    rng = np.random.default_rng([rows, rank])
+    gpu = pkg.Gpu(0)
+    try:
+        w, down, up = (gpu.bf16(bits(rng, width, width, std=width ** -0.5)), gpu.bf16(bits(rng, adapters, rank, width, std=width ** -0.5)),
+                       gpu.bf16(bits(rng, adapters, width, rank, std=0.1)))
+        key, value = gpu.bf16(bits(rng, states, width)), gpu.bf16(bits(rng, states, width))
+        start = bits(rng, rows, width)
+        maps = [gpu.u32(rng.integers(0, adapters + 1, rows).astype(np.uint32)) for _ in range(steps)]
+        tables = [gpu.u32(np.array([[0, rows, 0, 1 + 17 * i], [0, 0, 0, 0]], np.uint32).reshape(-1)) for i in range(steps)]
+        row_map, table = gpu.u32(np.zeros(rows, np.uint32)), gpu.u32(np.zeros(8, np.uint32))
+        x, y, z = (gpu.new(rows * width, pkg.BF16) for _ in range(3))
+        words = lambda t: gpu.wrap(t.pointer, t.elements, pkg.F32)          # for the copies
+
+        def run(drain):
+            x.write(start)
+            gpu.begin()
+
+            def op(*args):
+                gpu.op(*args)
+                if drain:
+                    gpu.submit()
+                    gpu.begin()
+            for i in range(steps):
+                op("copy_f32", words(row_map), 0, words(maps[i]), 0, rows)
+                op("h3x_linear_lora_bf16", y, x, w, None, down, up, None, row_map, rows, width, width, adapters, rank)
+                op("copy_f32", words(table), 0, words(tables[i]), 0, 8)
+                op("h3x_cross_sdpa_bf16", z, y, key, value, table, 2, rows, states, heads, heads, 128, 128 ** -0.5)
+                op("h3x_cross_sdpa_bf16", y, z, key, value, table, 2, rows, states, heads, heads, 128, 128 ** -0.5)
+                op("h3x_linear_lora_bf16", z, y, w, None, down, up, None, row_map, rows, width, width, adapters, rank)
+                op("add_bf16", x, x, z, rows * width)
+            gpu.submit()
+            return x.read()
+        want = run(True)
+        for _ in range(3):
+            assert np.array_equal(run(False), want)
+    finally:
+        gpu.close()
