@@ -348,18 +348,19 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         if (!*ring.stop) {
             /* rows part, part + split, ...: the row's own columns of all CTAs, scaled and rounded; zeros for the
              * entries that are not its own */
-            const uint32_t mine = (LR_M - part + split - 1) / split, pieces = task.rank8 / 4;
-            const uint32_t items = mine * (e1 - e0) * pieces;
-            for (uint32_t i = threadIdx.x; i < items; i += LR_THREADS) {
-                const uint32_t j = i % pieces * 4, e = e0 + i / pieces % (e1 - e0), r = part + i / pieces / (e1 - e0) * split;
-                if (row0 + r >= task.rows) continue;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (own[r] == e) {
-                    const uint32_t c = (e - e0) * args.rank16 + j;
+            const uint32_t mine = (LR_M - part + split - 1) / split, pieces = task.rank8 / 4, log2 = 32 - __clz(pieces - 1);
+            uint16_t *t_rows = task.t + (size_t(tile) * task.max_entries * task.tile_rows + row0 % task.tile_rows) * task.rank8;
+            for (uint32_t i = threadIdx.x; i < mine << log2; i += LR_THREADS) {
+                const uint32_t j = (i & ((1u << log2) - 1)) * 4, r = part + (i >> log2) * split;
+                if (j >= task.rank8 || row0 + r >= task.rows) continue;
+                const uint32_t e_own = own[r];
+                uint2 value = make_uint2(0, 0);
+                if (e_own - e0 < e1 - e0) {
+                    const uint32_t c = (e_own - e0) * args.rank16 + j;
                     const uint32_t at = ring.stage0 + (r * columns + ((c / 4) ^ (r & 3)) * 4) * 4;
-                    float4 x[LR_SPLIT];
+                    float4 x[LR_SPLIT], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (uint32_t p = 0; p < LR_SPLIT; p++)
+                    for (uint32_t p = 0; p < LR_SPLIT; p++)      /* all on the way before the first is used */
                         if (p < split)
                             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                                          : "=f"(x[p].x), "=f"(x[p].y), "=f"(x[p].z), "=f"(x[p].w) : "r"(cluster_map(at, p)) : "memory");
@@ -367,13 +368,11 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     for (uint32_t p = 0; p < LR_SPLIT; p++)
                         if (p < split) { v.x += x[p].x; v.y += x[p].y; v.z += x[p].z; v.w += x[p].w; }
                     const float s = own_scale[r];
-                    v.x = j < task.rank ? v.x * s : 0.0f;
-                    v.y = j + 1 < task.rank ? v.y * s : 0.0f;
-                    v.z = j + 2 < task.rank ? v.z * s : 0.0f;
-                    v.w = j + 3 < task.rank ? v.w * s : 0.0f;
+                    value = make_uint2(pack_bf16(j < task.rank ? v.x * s : 0.0f, j + 1 < task.rank ? v.y * s : 0.0f),
+                                       pack_bf16(j + 2 < task.rank ? v.z * s : 0.0f, j + 3 < task.rank ? v.w * s : 0.0f));
                 }
-                *reinterpret_cast<uint2 *>(task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + (row0 + r) % task.tile_rows) * task.rank8 + j) =
-                    make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                for (uint32_t e = e0; e < e1; e++)
+                    *reinterpret_cast<uint2 *>(t_rows + (size_t(e) * task.tile_rows + r) * task.rank8 + j) = e == e_own ? value : make_uint2(0, 0);
             }
         }
         /* nobody leaves, or loads over its shared memory, while that may be read */
