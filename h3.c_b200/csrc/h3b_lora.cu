@@ -847,7 +847,7 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
         /* room for every adapter in every tile; so many rows at a time that it stays within a gigabyte */
         const size_t tile_bytes = size_t(task.max_entries) * tile_rows * task.rank8 * 2;
         size_t chunk_tiles = (size_t(1) << 30) / tile_bytes;
-        if (chunk_tiles > 32768) chunk_tiles = 32768;          /* 128-row blocks are counted in a grid's y */
+        if (chunk_tiles > 32767) chunk_tiles = 32767;          /* two 128-row blocks each, counted in a grid's y */
         const size_t all_tiles = (size_t(rows) + tile_rows - 1) / tile_rows;
         if (chunk_tiles > all_tiles) chunk_tiles = all_tiles;
         const size_t t_bytes = rounded(chunk_tiles * tile_bytes);

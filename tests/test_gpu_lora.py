@@ -118,9 +118,12 @@ def test_low_rank_rows_beyond_a_gigabyte(gpu, pkg, rank):
     assert_within(case.run(gpu, pkg), *case.reference(), f"rank {rank}")
 
 
-@pytest.mark.parametrize("rows,k,n,rank", [(9_000_001, 8, 8, 8), (4_300_001, 3, 3, 2)])
-def test_more_rows_than_a_grid_dimension_holds(gpu, pkg, rows, k, n, rank):
-    """On the tensor cores and on the kernels for any shape; the input repeats a base block of rows."""
+@pytest.mark.parametrize("rows,k,n,rank,pairs", [(9_000_001, 8, 8, 8, False), (9_000_001, 8, 8, 8, True), (4_300_001, 3, 3, 2, False)])
+def test_more_rows_than_a_grid_dimension_holds(gpu, pkg, monkeypatch, rows, k, n, rank, pairs):
+    """On the tensor cores, with tiles of 128 and of 256 rows, and on the kernels for any shape; the input repeats a base
+    block of rows."""
+    if pairs:
+        monkeypatch.setenv("H3B_CTA_PAIRS_ALWAYS", "1")
     base = Case(1009, k, n, 3, rank, kind="random")
     want, tol = base.reference()
     tensors = base.tensors(gpu)
