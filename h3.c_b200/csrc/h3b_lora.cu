@@ -151,19 +151,22 @@ __device__ __forceinline__ uint32_t ring_tmem(const Ring &r) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(r.holder));
     return tmem;
 }
-__device__ __forceinline__ void ring_free(const RingArgs &args, uint32_t tmem) {
+/* Behind the last use of the accumulator: tensor memory goes back. After a wait that ran out: the status, and time for
+ * copies and products that may be in flight to land first. */
+__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r, uint32_t tmem) {
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*r.stop) {
+        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_GEMM_TIMEOUT));
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        __syncthreads();
+    }
     if (threadIdx.x >> 5 == 1) {
         tc_fence_after();
         tmem_free(tmem, args.tmem_columns);
     }
     __syncwarp();
-}
-/* a wait that ran out: the status, and time for copies that may be in flight to land */
-__device__ __forceinline__ void ring_close(const RingArgs &args, const Ring &r) {
-    if (*r.stop) {
-        if (threadIdx.x == 0) atomicMax(args.status, int(H3B_STATUS_GEMM_TIMEOUT));
-        for (int i = 0; i < 1000; i++) __nanosleep(1000);
-    }
 }
 
 /* The entries of a tile: the adapters that occur among its rows, ascending. Every CTA finds them for itself. */
@@ -380,11 +383,7 @@ h3b_lora_down_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         cluster_sync_all();
         tc_fence_after();
     }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    ring_free(args.ring, tmem);
-    ring_close(args.ring, ring);
+    ring_close(args.ring, ring, tmem);
     h3b_wait_for_launch();               /* the padded up rows, where a launch in front writes them: done before this one is */
 }
 
@@ -549,11 +548,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             }
         }
     }
-    /* tensor memory goes back while the cluster meets */
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    ring_free(args.ring, tmem);
+    ring_close(args.ring, ring, tmem);      /* tensor memory goes back while the cluster meets */
     cluster_sync_all();
     if (!*ring.stop && warp >= 2) {
         /* rows part, part + split, ... */
@@ -584,7 +579,6 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     }
     __syncwarp();
     cluster_sync_all();      /* nobody leaves while its shared memory may be read */
-    ring_close(args.ring, ring);
 }
 
 /* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes. 8 elements a thread. */
