@@ -427,7 +427,7 @@ h3b_lora_down_few(const __grid_constant__ h3b_lora_task task) {
     h3b_wait_for_launch();
 }
 
-/* The projection of few rows: D[weight row][x row] = W.x^T for 128 weight rows and a tile of up to 128 x rows, the
+/* The projection of few rows: D[weight row][x row] = W.x^T for 128 weight rows and the up to 128 rows of the call, the
  * weight streamed once through the M side of the instruction. K is split over the CTAs of a cluster so
  * that every SM pulls on the weight (42 weight tiles of n = 5,376 would leave 106 SMs idle); the last CTA
  * takes the entries' blocks too. Partial sums are joined through distributed shared memory in rank order.
@@ -445,8 +445,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     __shared__ int stop_flag;
     const h3b_lora_task &task = args.task;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t split = gridDim.x, part = blockIdx.x, w0 = blockIdx.y * LR_M, tile = blockIdx.z;
-    const uint32_t row0 = tile * task.tile_rows, live = min(task.tile_rows, task.rows - row0);
+    const uint32_t split = gridDim.x, part = blockIdx.x, w0 = blockIdx.y * LR_M;
     const uint32_t kb0 = part * args.k_blocks / split, kb1 = (part + 1) * args.k_blocks / split;
     const uint32_t b_bytes = task.tile_rows * LR_K * 2;
     Ring ring = ring_begin(args.ring, raw_smem, &stop_flag, 1);
@@ -478,7 +477,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 const uint32_t dst = next_stage(), bar = ring.full + 8 * stage;
                 if (!alive) break;
                 tma_load_2d(dst, &map_w, bar, int(kb * LR_K), int(w0));
-                tma_load_2d(dst + LR_A_BYTES, &map_x, bar, int(kb * LR_K), int(row0));
+                tma_load_2d(dst + LR_A_BYTES, &map_x, bar, int(kb * LR_K), 0);
                 advance();
             }
             alive = alive && mbar_wait(ring.info, 0, ring.stop, args.ring.wait_cycles);
@@ -488,7 +487,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 const uint32_t dst = next_stage(), bar = ring.full + 8 * stage;
                 if (!alive) break;
                 tma_load_3d(dst, &map_up, bar, int(c), int(w0), int(adapter[e]));
-                tma_load_2d(dst + LR_A_BYTES, &map_t, bar, int(c), int((tile * task.max_entries + e) * task.tile_rows));
+                tma_load_2d(dst + LR_A_BYTES, &map_t, bar, int(c), int(e * task.tile_rows));
                 advance();
             }
         }
@@ -520,8 +519,8 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         if (warp == 2) {
             /* what the launch in front found */
             h3b_wait_for_launch();
-            const uint32_t found = task.counts[tile], count = found & ~H3B_LORA_MIXED;
-            for (uint32_t e = lane; e < count; e += 32) adapter[e] = uint16_t(task.entries[size_t(tile) * task.max_entries + e]);
+            const uint32_t found = task.counts[0], count = found & ~H3B_LORA_MIXED;
+            for (uint32_t e = lane; e < count; e += 32) adapter[e] = uint16_t(task.entries[e]);
             if (lane == 0) {
                 entries = count;
                 rows_differ = found & H3B_LORA_MIXED;
@@ -533,7 +532,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         const uint32_t quarter = warp & 3;
         if (__all_sync(0xffffffffu, mbar_wait(ring.done, 0, ring.stop, args.ring.wait_cycles))) {
             tc_fence_after();
-            for (uint32_t c = 0; c < live; c += 16) {
+            for (uint32_t c = 0; c < task.rows; c += 16) {
                 uint32_t v[16];
                 asm volatile(
                     "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -556,7 +555,7 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         const bool mixed = rows_differ;
         if (col < task.n) {
             const float b0 = h3b_lo(bias), b1 = h3b_hi(bias);
-            for (uint32_t r = part + split * ((threadIdx.x >> 6) - 1); r < live; r += 2 * split) {
+            for (uint32_t r = part + split * ((threadIdx.x >> 6) - 1); r < task.rows; r += 2 * split) {
                 const uint32_t at = ring.stage0 + (r * LR_M + 2 * (threadIdx.x & 63)) * 4;
                 float v0 = 0.0f, v1 = 0.0f;
                 float x0[LR_SPLIT], x1[LR_SPLIT];
@@ -570,10 +569,10 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 v0 += b0;
                 v1 += b1;
                 if (mixed && (h3b_not_finite(v0) || h3b_not_finite(v1))) {
-                    v0 = h3b_lora_element(task, row0 + r, col);
-                    v1 = h3b_lora_element(task, row0 + r, col + 1);
+                    v0 = h3b_lora_element(task, r, col);
+                    v1 = h3b_lora_element(task, r, col + 1);
                 }
-                *reinterpret_cast<uint32_t *>(task.out + size_t(row0 + r) * task.n + col) = pack_bf16(v0, v1);
+                *reinterpret_cast<uint32_t *>(task.out + size_t(r) * task.n + col) = pack_bf16(v0, v1);
             }
         }
     }
@@ -717,7 +716,7 @@ uint32_t split_for(h3_gpu *gpu, Kernel *kernel, size_t smem, uint32_t per_sm, ui
 int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool captured) {
     const bool dependent = !captured || !task.first;
     const uint32_t k_blocks = (task.k + LR_K - 1) / LR_K;
-    const uint32_t tiles = (task.rows + task.tile_rows - 1) / task.tile_rows, row_blocks = (task.rows + LR_M - 1) / LR_M;
+    const uint32_t row_blocks = (task.rows + LR_M - 1) / LR_M;
     CUtensorMap map_x, map_down;
     DownArgs down = {};
     down.task = task;
@@ -747,8 +746,12 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
     if (!lora_map(&map_x, task.x, task.rows, task.k, LR_M) ||
         !lora_map(&map_down, task.down, uint64_t(task.adapters) * task.rank, task.k, down.rank16))
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
-    /* by warps while that reads the inputs a few times at most from L2 */
-    if (few && task.rows <= uint32_t(LR_M) && uint64_t(task.rows) * task.rank <= 2048)
+    /* By warps where that is the shorter way and there is no long weight stream to hide it behind (us, by warps / tensor
+     * cores: 4 rows 1,024 -> 5,376 rank 16 8.6 / 11.7, 128 rows 15.1 / 17.5, rank 64 22.2 / 18.5; 2,048 -> 5,376 16
+     * rows 12.0 / 13.3; 2,688 -> 10,752 16 rows 18.9 / 17.0; 5,376 -> 5,376 64 rows 21.8 / 19.5), and for the smallest
+     * calls of all (1 row 5,376 -> 5,376 rank 16 16.0 / 16.8). */
+    const uint64_t sums = uint64_t(task.rows) * task.rank;
+    if (few && (sums <= 16 || (sums <= 2048 && uint64_t(task.n) * task.k <= 12000000)))
         launch_cluster(gpu, h3b_lora_down_few, dim3(task.rows, task.rank8 / LF_SUMS), 32 * LF_WARPS, 1, 0, dependent, task);
     else
         launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, side), LR_THREADS, down_split, ring_smem(down.ring), dependent,
@@ -769,7 +772,7 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
     rows.ring.stages = (106 << 10) / rows.ring.stage_bytes;
     if (rows.ring.stages > uint32_t(LR_STAGES)) rows.ring.stages = LR_STAGES;
     const uint32_t weight_tiles = (task.n + LR_M - 1) / LR_M;
-    const uint32_t split = split_for(gpu, h3b_lora_rows, ring_smem(rows.ring), 2, uint64_t(weight_tiles) * tiles, k_blocks);
+    const uint32_t split = split_for(gpu, h3b_lora_rows, ring_smem(rows.ring), 2, weight_tiles, k_blocks);
     CUtensorMap map_w, map_rows, map_up, map_t;
     EncodeTiled encode = encode_tiled();
     cuuint64_t dims[3] = {task.rank8, task.n, task.adapters};
@@ -777,12 +780,12 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
     cuuint32_t box[3] = {LR_K, LR_M, 1};
     cuuint32_t elem[3] = {1, 1, 1};
     if (!lora_map(&map_w, task.w, task.n, task.k, LR_M) || !lora_map(&map_rows, task.x, task.rows, task.k, task.tile_rows) ||
-        !lora_map(&map_t, task.t, uint64_t(tiles) * task.max_entries * task.tile_rows, task.rank8, task.tile_rows) ||
+        !lora_map(&map_t, task.t, uint64_t(task.max_entries) * task.tile_rows, task.rank8, task.tile_rows) ||
         encode(&map_up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(task.up8), dims, strides, box, elem,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
-    launch_cluster(gpu, h3b_lora_rows, dim3(split, weight_tiles, tiles), LR_THREADS, split, ring_smem(rows.ring), true, map_w, map_rows, map_up, map_t, rows);
+    launch_cluster(gpu, h3b_lora_rows, dim3(split, weight_tiles), LR_THREADS, split, ring_smem(rows.ring), true, map_w, map_rows, map_up, map_t, rows);
     return 1;
 }
 
@@ -830,10 +833,12 @@ extern "C" int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3
         task.out = y;
         task.rows = rows; task.k = input_dim; task.n = output_dim; task.adapters = adapters; task.rank = rank;
         task.rank8 = (rank + 7) & ~7u;
-        /* The weight-streaming kernel while one row tile covers the call and the GEMM's tiles would leave SMs idle.
-         * 5,376 -> 5,376, GEMM / streaming: 16 rows 62 / 31 us, 64 54 / 37, 128 54 / 36, 200 42 / 53, 512 40 / 55;
-         * 42 rows 2,688 -> 96,768 (378 GEMM tiles) 105 / 110. */
-        const bool few = rows <= uint32_t(LR_M) && uint64_t((output_dim + 255) / 256) < uint64_t(gpu->sm_count);
+        /* The weight-streaming kernel takes calls of one row tile: up to 16 rows of any width, and more while the GEMM's tiles
+         * would leave two thirds of the SMs idle (us, streaming / GEMM, 5,376 and 2,688 inputs: 1 row -> 21,504 43.8 / 59.6,
+         * 25.6 / 34.1; 16 rows -> 28,672 53.5 / 53.7, 31.4 / 36.9, -> 96,768 164 / 164, 91 / 111; 100 rows -> 5,376 22 / 39
+         * (5,376), -> 10,752 30.5 / 41.2, 21.2 / 25.5, -> 16,384 41.2 / 43.2, 27.3 / 26.0, -> 21,504 58.7 / 47.6, 37.8 / 29.3) */
+        const uint64_t gemm_tiles = (uint64_t(output_dim) + 255) / 256;
+        const bool few = (rows <= 16 && gemm_tiles < 32768) || (rows <= uint32_t(LR_M) && 3 * gemm_tiles <= uint64_t(gpu->sm_count));
         const uint32_t tile_rows = few ? (rows + 15) & ~15u : h3b_gemm_lora_tile_rows(gpu, rows, output_dim);
         task.tile_rows = tile_rows;
         task.max_entries = adapters < tile_rows ? adapters : tile_rows;

@@ -111,6 +111,14 @@ def test_more_adapters_than_are_computed_side_by_side(gpu, pkg, rows, k, n, adap
     assert_within(case.run(gpu, pkg), *case.reference(), f"{case.sizes()}")
 
 
+@pytest.mark.parametrize("rows,k,n,adapters,rank", [
+    (1, 264, 50008, 3, 12), (9, 328, 38000, 4, 16), (16, 128, 100008, 2, 8), (17, 128, 100008, 2, 8), (2, 2816, 12552, 3, 24),
+    (1, 8, 2_200_000, 2, 8), (3, 8, 8_400_000, 2, 8)])
+def test_few_rows_of_a_wide_projection(gpu, pkg, rows, k, n, adapters, rank):
+    case = Case(rows, k, n, adapters, rank, kind="random")
+    assert_within(case.run(gpu, pkg), *case.reference(), f"{case.sizes()}")
+
+
 @pytest.mark.parametrize("rank", [256, 250])
 def test_low_rank_rows_beyond_a_gigabyte(gpu, pkg, rank):
     """256 entries of 256 rows in every tile: the rows are taken in several passes."""
