@@ -147,3 +147,54 @@ def test_a_chain_of_calls_equals_the_calls_one_by_one(pkg, rows, rank):
             assert np.array_equal(run(False), want)
     finally:
         gpu.close()
+
+
+def test_two_contexts_at_once(pkg):
+    """Calls of every kind in two contexts on two streams, interleaved without a wait: the bits of each on its own."""
+    import torch
+    rng = np.random.default_rng(5)
+    contexts = [pkg.Gpu(0), pkg.Gpu(0)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    try:
+        calls = []          # per context: (name, arguments, output)
+        for gpu, stream in zip(contexts, streams):
+            gpu.set_stream(stream.cuda_stream)
+            mine = []
+            for rows, k, n, adapters, rank in ((640, 1024, 1536, 3, 16), (3, 1024, 1024, 3, 8), (100, 2048, 1024, 3, 64), (300, 1000, 520, 2, 12)):
+                out = gpu.new(rows * n, pkg.BF16)
+                mine.append(("h3x_linear_lora_bf16", (out, gpu.bf16(bits(rng, rows, k)), gpu.bf16(bits(rng, n, k, std=k ** -0.5)), None,
+                                                      gpu.bf16(bits(rng, adapters, rank, k, std=k ** -0.5)),
+                                                      gpu.bf16(bits(rng, adapters, n, rank, std=0.1)), None,
+                                                      gpu.u32(rng.integers(0, adapters + 1, rows).astype(np.uint32)), rows, k, n,
+                                                      adapters, rank), out))
+            for segments, heads, kv_heads, dim in (([[0, 700, 0, 300], [700, 90, 300, 77]], 8, 8, 128), ([[0, 1, 0, 2000], [1, 1, 40, 5]], 8, 2, 128),
+                                                   ([[0, 400, 0, 260]], 6, 6, 64)):
+                rows, keys = max(s[0] + s[1] for s in segments), max(s[2] + s[3] for s in segments)
+                out = gpu.new(rows * heads * dim, pkg.BF16)
+                mine.append(("h3x_cross_sdpa_bf16", (out, gpu.bf16(bits(rng, rows, heads * dim)), gpu.bf16(bits(rng, keys, kv_heads * dim)),
+                                                     gpu.bf16(bits(rng, keys, kv_heads * dim)),
+                                                     gpu.u32(np.array(segments, np.uint32).reshape(-1)), len(segments), rows, keys, heads,
+                                                     kv_heads, dim, dim ** -0.5), out))
+            calls.append(mine)
+        want = []
+        for gpu, mine in zip(contexts, calls):
+            gpu.begin()
+            for name, args, _ in mine:
+                gpu.op(name, *args)
+            gpu.submit()
+            want.append([out.read() for _, _, out in mine])
+        for gpu in contexts:
+            gpu.begin()
+        for turn in range(30):
+            for i in range(len(calls[0])):
+                for c, gpu in enumerate(contexts):
+                    name, args, _ = calls[c][(i + 3 * c + turn) % len(calls[c])]
+                    gpu.op(name, *args)
+        for gpu in contexts:
+            gpu.submit()
+        for c in range(2):
+            for (name, _, out), bits_alone in zip(calls[c], want[c]):
+                assert np.array_equal(out.read(), bits_alone), name
+    finally:
+        for gpu in contexts:
+            gpu.close()
