@@ -563,12 +563,42 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 have = cursor.next(args, u);
                 continue;
             }
+            auto clear_tail = [&](uint32_t j) {
+                if (!u.dirty || j + 1 != steps || g != 0) return;
+                /* value rows that are not the segment's: cleared before anybody's P.V, which is issued
+                 * behind this group's arrival */
+                const bool ok = __all_sync(0xffffffffu, mbar_wait(tail + 8 * (t & 1u), tail_phase >> (t & 1u) & 1u, stop, budget));
+                if (ok && local_row >= u.keys - j * CT) {
+                    const uint32_t at = v_smem + (t % STAGES) * TILE + local_row * 128 + (D == 128 ? half * CT_BOX : half * 64);
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + i * 16), "r"(0) : "memory");
+                }
+                fence_async_smem();
+                tail_phase ^= 1u << (t & 1u);
+            };
+            /* None of the warp's rows is the segment's: whatever its scores make of its rows of O is stored by nobody, and the
+             * others have the exponentials to themselves (64 rows of 300 keys each x 56 heads 121.5 us, 129.4 with
+             * the dead rows; 8 x 1,000 keys, dim 64 20.9, 22.6; a ragged batch 76.3, 78.0). */
+            const bool idle = g * tile_rows + ((quarter * 32) >> args.pack_log2) >= u.rows;
             float reference = -INFINITY, sum = 0.0f;
             for (uint32_t j = 0; j < steps; j++, t++) {
-                bool ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, t & 1u, stop, budget));
+                const bool ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * g, t & 1u, stop, budget));
                 tc_fence_after();
                 /* the last group's scores are the last to be complete: the stage before is free */
                 if (g == GROUPS - 1 && half == 0 && quarter == 0 && lane == 0) mbar_arrive(seen + 8 * (t & 1u));
+                if (idle) {
+                    alive = meet(ok);
+                    if (!alive) break;
+                    clear_tail(j);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(go + 16 * g + 8 * (t & 1u));
+                        mbar_arrive(go2 + 16 * g + 8 * (t & 1u));
+                    }
+                    continue;
+                }
                 const int valid = int(min(u.keys - j * CT, uint32_t(CT))) - int(half * 64);
                 /* 32 scores at a time, read from tensor memory twice (for the maximum, for the exponentials):
                  * holding all 64 spills at the 96 registers there are for 18 warps */
@@ -622,19 +652,7 @@ h3b_cross_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                 const float neg_m = reference == -INFINITY ? 0.0f : -reference;
                 const uint64_t neg_m2 = pack_f32x2(neg_m, neg_m);
                 uint64_t sum_a = 0, sum_b = 0;
-                if (u.dirty && j + 1 == steps && g == 0) {
-                    /* value rows that are not the segment's: cleared before anybody's P.V, which is issued
-                     * behind this group's arrival */
-                    ok = __all_sync(0xffffffffu, mbar_wait(tail + 8 * (t & 1u), tail_phase >> (t & 1u) & 1u, stop, budget));
-                    if (ok && local_row >= u.keys - j * CT) {
-                        const uint32_t at = v_smem + (t % STAGES) * TILE + local_row * 128 + (D == 128 ? half * CT_BOX : half * 64);
-#pragma unroll
-                        for (int i = 0; i < D / 16; i++)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + i * 16), "r"(0) : "memory");
-                    }
-                    fence_async_smem();
-                    tail_phase ^= 1u << (t & 1u);
-                }
+                clear_tail(j);
                 /* P of 32 keys lands on columns in front of the scores that are still to be read */
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
