@@ -802,22 +802,20 @@ h3b_cross_merge(const CrossArgs args) {
     for (uint32_t s0 = 0; s0 < pieces; s0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.0f);
         if (s0 + lane < pieces) ml = *reinterpret_cast<const float2 *>(args.partial_ml + ((s0 + lane) * all + unit) * 2);
-        /* a part that attended nothing has no rows written */
-        const bool used = !(ml.x == -INFINITY && ml.y == 0.0f);
-        const float weight = used ? ct_exp2(ml.x - most) : 0.0f;
-        float part = used ? ml.y * weight : 0.0f;
+        /* A piece without a score above -inf: weight 0, not 2^(-inf + inf). Its rows take part all the same: they are
+         * zeros, and NaN where a value is not finite, as 0 times it is in a segment in one piece. */
+        const float weight = ml.x == -INFINITY ? 0.0f : ct_exp2(ml.x - most);
+        float part = ml.y * weight;
 #pragma unroll
         for (int q = 16; q; q >>= 1) part += __shfl_xor_sync(0xffffffffu, part, q);
         sum += part;
-        const uint32_t used_mask = __ballot_sync(0xffffffffu, used), count = min(32u, pieces - s0);
+        const uint32_t count = min(32u, pieces - s0);
 #pragma unroll 8
         for (uint32_t s = 0; s < count; s++) {
             const Vector v = reinterpret_cast<const Vector *>(args.partial_o + ((s0 + s) * all + unit) * D)[lane];
             const float w = __shfl_sync(0xffffffffu, weight, s);
-            if (used_mask >> s & 1u) {
 #pragma unroll
-                for (int i = 0; i < PER; i++) o[i] = fmaf(reinterpret_cast<const float *>(&v)[i], w, o[i]);
-            }
+            for (int i = 0; i < PER; i++) o[i] = fmaf(reinterpret_cast<const float *>(&v)[i], w, o[i]);
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
