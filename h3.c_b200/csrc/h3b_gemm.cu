@@ -54,6 +54,7 @@ constexpr int STAGES = 4;
 constexpr int A_BYTES = BM * BK * 2;   /* 16 KiB */
 constexpr int B_BYTES = BN * BK * 2;   /* 32 KiB */
 constexpr int TC_THREADS = 192;
+static_assert(TC_THREADS == int(H3B_LORA_THREADS), "the repair of adapter tiles is written for it");
 constexpr size_t TC_SMEM = size_t(STAGES) * (A_BYTES + B_BYTES) + 1024 /*align*/ + 256 /*barriers*/;
 /* the QKV epilogue turns its row-per-thread results into whole-row stores through an
  * 8 KiB staging area per epilogue warp */
@@ -344,11 +345,13 @@ __device__ __noinline__ bool split_tile_merge(const SplitCall args, uint32_t lan
 }
 
 /* One thread's share of a finished 128 x 256 accumulator tile: its row (TMEM lane) through the
- * epilogue EPI. lane_addr = TMEM address of the row's first column. */
+ * epilogue EPI. lane_addr = TMEM address of the row's first column. Returns whether an adapter tile has
+ * something to be repaired (h3b_lora_repair). */
 template <int EPI>
-__device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_addr, uint32_t row,
+__device__ __forceinline__ bool tile_epilogue(const TcArgs &args, uint32_t lane_addr, uint32_t row,
                                               bool row_ok, uint32_t n_blk, uint32_t stage_smem,
                                               uint32_t lane, const Extra<EPI> &extra) {
+                bool repair = false;
                 if (EPI == H3B_EPI_QKV_ROPE) {
                     /* the tile's 256 columns are two whole 128-column units of the grouped row */
     #pragma unroll 1
@@ -468,21 +471,12 @@ __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_
                         }
                         if constexpr (EPI == H3B_EPI_LORA) {
                             /* Something not finite (times zero: NaN, found once for 32 columns): maybe another row's
-                             * adapter (see h3b_lora_element). A test and branch per pair cost 1,003 rows x 5,376
+                             * adapter (see h3b_lora_repair). A test and branch per pair cost 1,003 rows x 5,376
                              * columns 6 us. */
                             float zero = 0.0f;
     #pragma unroll
                             for (int i = 0; i < 32; i++) zero = fmaf(__uint_as_float(r[i]), 0.0f, zero);
-                            if (mixed && zero != 0.0f) {
-    #pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    float lo = __uint_as_float(r[2 * i]), hi = __uint_as_float(r[2 * i + 1]);
-                                    const uint32_t col = col0 + 2 * i;
-                                    if ((h3b_not_finite(lo) || h3b_not_finite(hi)) && col < args.out_cols)
-                                        packed[i] = pack_bf16(h3b_lora_element(extra.task, row, col),
-                                                              h3b_lora_element(extra.task, row, col + 1));
-                                }
-                            }
+                            repair |= mixed && zero != 0.0f;
                         }
                         if (row_ok) {
     #pragma unroll
@@ -494,6 +488,7 @@ __device__ __forceinline__ void tile_epilogue(const TcArgs &args, uint32_t lane_
                         }
                     }
                 }
+                return repair;
 }
 
 /* a box of an adapter's up matrix (z = adapter) */
@@ -548,6 +543,7 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     tc_fence_after();
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_holder));
+    bool repair = false;         /* adapter epilogue: something of this thread's rows has to be computed again */
 
     const uint32_t group_tiles = args.group_m * args.tiles_n;
 
@@ -682,8 +678,8 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 split_tile_merge(SplitCall{args.split_scratch, args.split_counters, args.wait_cycles,
                                            args.split_tiles, args.split, item.slot, item.part},
                                  lane_addr, quarter * 32 + lane, BM, 4, lane, stop))
-                tile_epilogue<EPI>(args, lane_addr, row, row_ok, n_blk,
-                                   bars + 256 + quarter * QKV_STAGE_BYTES, lane, extra);
+                repair |= tile_epilogue<EPI>(args, lane_addr, row, row_ok, n_blk,
+                                             bars + 256 + quarter * QKV_STAGE_BYTES, lane, extra);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
@@ -704,6 +700,18 @@ h3b_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         tc_fence_after();
         tmem_free(tmem_base, 512);
     }
+    if constexpr (EPI == H3B_EPI_LORA)
+        if (__syncthreads_or(repair)) {
+            h3b_wait_for_launch();
+            WorkItem item;
+            for (uint32_t pass = 0; next_item(args, blockIdx.x, gridDim.x, pass, item); pass++) {
+                uint32_t m_blk, n_blk;
+                tile_coords(item.tile, m_blk, n_blk);
+                if (item.part == 0 && (extra.task.counts[m_blk] & H3B_LORA_MIXED))
+                    h3b_lora_repair(extra.task, reinterpret_cast<float *>(raw_smem + (base - smem_u32(raw_smem))), m_blk * BM, 1,
+                                    min(uint32_t(BM), args.rows - m_blk * BM), n_blk * BN, min(uint32_t(BN), args.out_cols - n_blk * BN));
+            }
+        }
 }
 
 /* ---- the same GEMM on CTA pairs ------------------------------------------------------
@@ -772,6 +780,7 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_holder));
 
+    bool repair = false;
     /* tiles_m counts 256-row tiles */
     const uint32_t group_tiles = args.group_m * args.tiles_n;
     auto tile_coords = [&](uint32_t tile, uint32_t &m_blk, uint32_t &n_blk) {
@@ -895,8 +904,8 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 split_tile_merge(SplitCall{args.split_scratch, args.split_counters, args.wait_cycles,
                                            args.split_tiles, args.split, item.slot, item.part},
                                  lane_addr, rank * BM + quarter * 32 + lane, 2 * BM, 8, lane, stop))
-                tile_epilogue<EPI>(args, lane_addr, row, row < args.rows, n_blk,
-                                   bars + 256 + quarter * QKV_STAGE_BYTES, lane, extra);
+                repair |= tile_epilogue<EPI>(args, lane_addr, row, row < args.rows, n_blk,
+                                             bars + 256 + quarter * QKV_STAGE_BYTES, lane, extra);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(cluster_map(acc_empty + 8 * acc, 0));
@@ -919,6 +928,19 @@ h3b_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         tc_fence_after();
         tmem_free_pair(tmem_base, 512);
     }
+    if constexpr (EPI == H3B_EPI_LORA)
+        if (__syncthreads_or(repair)) {          /* each CTA its own rows */
+            h3b_wait_for_launch();
+            WorkItem item;
+            for (uint32_t pass = 0; next_item(args, pair, pairs, pass, item); pass++) {
+                uint32_t m_blk, n_blk;
+                tile_coords(item.tile, m_blk, n_blk);
+                const uint32_t row0 = m_blk * 2 * BM + rank * BM;
+                if (item.part == 0 && row0 < args.rows && (extra.task.counts[m_blk] & H3B_LORA_MIXED))
+                    h3b_lora_repair(extra.task, reinterpret_cast<float *>(raw_smem + (base - smem_u32(raw_smem))), row0, 1,
+                                    min(uint32_t(BM), args.rows - row0), n_blk * BN, min(uint32_t(BN), args.out_cols - n_blk * BN));
+            }
+        }
 }
 
 /* ------------------------------------------------------------- SIMT GEMM */

@@ -100,6 +100,7 @@ constexpr int LR_M = 128;                    /* rows of an instruction: x rows (
 constexpr int LR_K = 64;                     /* one 128-byte swizzle line */
 constexpr int LR_A_BYTES = LR_M * LR_K * 2;
 constexpr int LR_THREADS = 192;              /* TMA, MMA, 4 epilogue warps */
+static_assert(LR_THREADS == int(H3B_LORA_THREADS), "the repair of adapter tiles is written for it");
 constexpr uint32_t LR_SPLIT = 8;             /* CTAs of a cluster, at most */
 constexpr int LR_STAGES = 8;                 /* barriers laid out; a launch uses `stages` of them */
 constexpr int LR_BAR_BYTES = 256;
@@ -549,9 +550,9 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     }
     ring_close(args.ring, ring, tmem);      /* tensor memory goes back while the cluster meets */
     cluster_sync_all();
+    bool repair = false;
     if (!*ring.stop && warp >= 2) {
         /* rows part, part + split, ... */
-        h3b_wait_for_launch();               /* the recomputed elements read what the launch in front wrote */
         const bool mixed = rows_differ;
         if (col < task.n) {
             const float b0 = h3b_lo(bias), b1 = h3b_hi(bias);
@@ -568,16 +569,18 @@ h3b_lora_rows(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     if (p < split) { v0 += x0[p]; v1 += x1[p]; }
                 v0 += b0;
                 v1 += b1;
-                if (mixed && (h3b_not_finite(v0) || h3b_not_finite(v1))) {
-                    v0 = h3b_lora_element(task, r, col);
-                    v1 = h3b_lora_element(task, r, col + 1);
-                }
+                repair |= mixed && (h3b_not_finite(v0) || h3b_not_finite(v1));
                 *reinterpret_cast<uint32_t *>(task.out + size_t(r) * task.n + col) = pack_bf16(v0, v1);
             }
         }
     }
     __syncwarp();
-    cluster_sync_all();      /* nobody leaves while its shared memory may be read */
+    cluster_sync_all();      /* nobody leaves, or writes over its shared memory, while that may be read */
+    if (__syncthreads_or(repair)) {
+        h3b_wait_for_launch();
+        h3b_lora_repair(task, reinterpret_cast<float *>(raw_smem + (ring.stage0 - smem_u32(raw_smem))), part, split,
+                        (task.rows - part + split - 1) / split, w0, min(uint32_t(LR_M), task.n - w0));
+    }
 }
 
 /* up with rows of rank8 elements, zeros behind the rank: TMA wants row strides of 16 bytes. 8 elements a thread. */

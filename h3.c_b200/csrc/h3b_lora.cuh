@@ -33,21 +33,104 @@ int h3b_gemm_lora(h3_gpu *gpu, const h3b_lora_task &task, bool captured);
 
 #ifdef __CUDACC__
 /* In a tile whose rows differ in their adapter, a row meets the other adapters' up rows times zeros. Where
- * those are not finite the accumulator is NaN although the row's own result may be finite: such an element
- * is computed again on its own, in F32, from its row's adapter alone. */
-static __device__ __noinline__ float h3b_lora_element(const h3b_lora_task &task, uint32_t row, uint32_t col) {
-    float v = task.bias ? h3b_widen(task.bias[col]) : 0.0f;
-    const uint16_t *x = task.x + size_t(row) * task.k, *w = task.w + size_t(col) * task.k;
-    for (uint32_t i = 0; i < task.k; i++) v = fmaf(h3b_widen(x[i]), h3b_widen(w[i]), v);
-    const uint32_t a = task.row_adapter ? task.row_adapter[row] : 0, tile = row / task.tile_rows;
-    const uint32_t count = a < task.adapters ? task.counts[tile] & ~H3B_LORA_MIXED : 0;
-    for (uint32_t e = 0; e < count; e++)
-        if (task.entries[size_t(tile) * task.max_entries + e] == a) {
-            const uint16_t *t = task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + row % task.tile_rows) * task.rank8;
-            const uint16_t *u = task.up + (size_t(a) * task.n + col) * task.rank;
-            for (uint32_t j = 0; j < task.rank; j++) v = fmaf(h3b_widen(t[j]), h3b_widen(u[j]), v);
+ * those are not finite the accumulator is NaN although the row's own result may be finite. Such a tile is stored as it
+ * comes, and behind its last tile, where no wait of the kernel runs any more, the CTA that stored it computes what is
+ * not finite in it again, from each row's own adapter alone: F32 chains over k and then the rank, 64 x 64 outputs at a
+ * time, 8 x 4 of them a thread, both operands through shared memory (one element at a time, inside the epilogue,
+ * 400 rows 7,168 -> 768 of three adapters, one of infinities, took 139 ms and held up the accumulators' waits). */
+constexpr uint32_t H3B_LORA_THREADS = 192, H3B_LORA_REPAIR_K = 32, H3B_LORA_REPAIR_PITCH = 68;
+/* Rows row0, row0 + stride, ... (`count` of them) of output columns col0 .. col0 + columns - 1, by all threads of the CTA;
+ * smem: 2 * 32 * 68 floats, 16-byte aligned. */
+static __device__ __noinline__ void h3b_lora_repair(const h3b_lora_task &task, float *smem, uint32_t row0, uint32_t stride,
+                                                    uint32_t count, uint32_t col0, uint32_t columns) {
+    constexpr uint32_t SIDE = 64, K = H3B_LORA_REPAIR_K, PITCH = H3B_LORA_REPAIR_PITCH, PIECES = 2 * SIDE * K / 8;
+    constexpr uint32_t LOADS = (PIECES + H3B_LORA_THREADS - 1) / H3B_LORA_THREADS;
+    const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;      /* ty 8 and up: loads only */
+    for (uint32_t r0 = 0; r0 < count; r0 += SIDE)
+        for (uint32_t c0 = 0; c0 < columns; c0 += SIDE) {
+            const uint32_t col = col0 + c0 + 4 * tx;
+            uint32_t bad = 0;                                         /* bit 4 i + j: row i, column j of the thread's */
+            if (ty < 8 && c0 + 4 * tx < columns)
+                for (uint32_t i = 0; i < 8 && r0 + 8 * ty + i < count; i++) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(task.out + size_t(row0 + (r0 + 8 * ty + i) * stride) * task.n + col);
+                    const uint32_t words[2] = {v.x, v.y};
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) bad |= uint32_t((words[j / 2] >> (16 * (j & 1)) & 0x7f80u) == 0x7f80u) << (4 * i + j);
+                }
+            if (!__syncthreads_or(bad != 0)) continue;
+            float acc[8][4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const float start = task.bias && c0 + 4 * tx < columns ? h3b_widen(task.bias[col + j]) : 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) acc[i][j] = start;
+            }
+            /* 8 values of k at a time (k is a multiple of 8): piece p is of x (p < 256) or w, row p & 63 */
+            uint4 next[LOADS];
+            auto load = [&](uint32_t k0) {
+#pragma unroll
+                for (uint32_t l = 0; l < LOADS; l++) {
+                    const uint32_t p = threadIdx.x + l * H3B_LORA_THREADS, r = p & (SIDE - 1), k = k0 + 8 * (p / SIDE & 3);
+                    next[l] = make_uint4(0, 0, 0, 0);
+                    if (p >= PIECES || k >= task.k) continue;
+                    if (p < PIECES / 2) {
+                        if (r0 + r < count) next[l] = *reinterpret_cast<const uint4 *>(task.x + size_t(row0 + (r0 + r) * stride) * task.k + k);
+                    } else if (c0 + r < columns) {
+                        next[l] = *reinterpret_cast<const uint4 *>(task.w + size_t(col0 + c0 + r) * task.k + k);
+                    }
+                }
+            };
+            load(0);
+            for (uint32_t k0 = 0; k0 < task.k; k0 += K) {
+#pragma unroll
+                for (uint32_t l = 0; l < LOADS; l++) {
+                    const uint32_t p = threadIdx.x + l * H3B_LORA_THREADS;
+                    if (p >= PIECES) break;
+                    float *at = smem + (p < PIECES / 2 ? 0 : K * PITCH) + 8 * (p / SIDE & 3) * PITCH + (p & (SIDE - 1));
+                    const uint32_t words[4] = {next[l].x, next[l].y, next[l].z, next[l].w};
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; q++) {
+                        at[2 * q * PITCH] = h3b_lo(words[q]);
+                        at[(2 * q + 1) * PITCH] = h3b_hi(words[q]);
+                    }
+                }
+                __syncthreads();
+                if (k0 + K < task.k) load(k0 + K);
+                if (ty < 8) {
+#pragma unroll 4
+                    for (uint32_t k = 0; k < K; k++) {
+                        const float4 a0 = *reinterpret_cast<const float4 *>(smem + k * PITCH + 8 * ty);
+                        const float4 a1 = *reinterpret_cast<const float4 *>(smem + k * PITCH + 8 * ty + 4);
+                        const float4 b = *reinterpret_cast<const float4 *>(smem + (K + k) * PITCH + 4 * tx);
+                        const float as[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; i++)
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) acc[i][j] = fmaf(as[i], bs[j], acc[i][j]);
+                    }
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                if (!(bad >> (4 * i) & 15u)) continue;
+                const uint32_t row = row0 + (r0 + 8 * ty + i) * stride, tile = row / task.tile_rows;
+                const uint32_t a = task.row_adapter ? task.row_adapter[row] : 0;
+                const uint32_t entries = a < task.adapters ? task.counts[tile] & ~H3B_LORA_MIXED : 0;
+                for (uint32_t e = 0; e < entries; e++) {
+                    if (task.entries[size_t(tile) * task.max_entries + e] != a) continue;
+                    const uint16_t *t = task.t + ((size_t(tile) * task.max_entries + e) * task.tile_rows + row % task.tile_rows) * task.rank8;
+                    const uint16_t *u = task.up + (size_t(a) * task.n + col) * task.rank;
+                    for (uint32_t q = 0; q < task.rank; q++)
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) acc[i][j] = fmaf(h3b_widen(t[q]), h3b_widen(u[size_t(j) * task.rank + q]), acc[i][j]);
+                    break;
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if (bad >> (4 * i + j) & 1u) task.out[size_t(row) * task.n + col + j] = __bfloat16_as_ushort(__float2bfloat16_rn(acc[i][j]));
+            }
         }
-    return v;
 }
 __device__ __forceinline__ bool h3b_not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 
