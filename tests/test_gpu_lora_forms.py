@@ -52,3 +52,37 @@ def test_an_adapter_of_infinities_holds_up_no_wait(pkg, rows, k, n):
         check_beside_infinities(gpu, pkg, Case(rows, k, n, 3, 16, kind="random"))
     finally:
         gpu.close()
+
+
+# ------------------------------------------------------------------ the last round of tiles split along k
+# 1,003 rows x 5,376 columns are 84 tiles of 256 x 256 on 74 pairs of SMs, or 168 of 128 x 256 on 148: what is left over
+# after a round is cut along k into as many slices as there are 8 K blocks of 64, four at most, and the last slice
+# carries the adapters. 400 rows x 38,400 are 300 pair tiles: four whole rounds in front.
+
+SPLIT = [(1003, 2048, 5376, 16, 12), (1003, 1536, 5376, 5, 64), (1003, 1024, 5376, 3, 100), (400, 1024, 38400, 3, 16)]
+
+
+@pytest.mark.parametrize("pairs", [True, False])
+@pytest.mark.parametrize("kind", ["runs", "each", "none"])
+@pytest.mark.parametrize("rows,k,n,adapters,rank", SPLIT)
+def test_the_split_last_round(gpu, pkg, monkeypatch, rows, k, n, adapters, rank, kind, pairs):
+    if not pairs:
+        monkeypatch.setenv("H3B_NO_CTA_PAIRS", "1")
+    case = Case(rows, k, n, adapters, rank, kind=kind)
+    want, tol = case.reference()
+    got = case.run(gpu, pkg)
+    assert_within(got, want, tol, f"{case.sizes()}")
+    assert np.array_equal(got, case.run(gpu, pkg))
+    # other sums in another order: this shape did split, and without it the same holds
+    monkeypatch.setenv("H3B_NO_SPLIT_K", "1")
+    whole = case.run(gpu, pkg)
+    assert_within(whole, want, tol, f"whole {case.sizes()}")
+    assert not np.array_equal(got, whole)
+
+
+@pytest.mark.parametrize("pairs", [True, False])
+@pytest.mark.parametrize("rows,k,n,adapters,rank", [SPLIT[0], SPLIT[2]])
+def test_the_split_last_round_beside_infinities(gpu, pkg, monkeypatch, rows, k, n, adapters, rank, pairs):
+    if not pairs:
+        monkeypatch.setenv("H3B_NO_CTA_PAIRS", "1")
+    check_beside_infinities(gpu, pkg, Case(rows, k, n, adapters, rank, kind="each"))
