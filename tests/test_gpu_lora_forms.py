@@ -86,3 +86,16 @@ def test_the_split_last_round_beside_infinities(gpu, pkg, monkeypatch, rows, k, 
     if not pairs:
         monkeypatch.setenv("H3B_NO_CTA_PAIRS", "1")
     check_beside_infinities(gpu, pkg, Case(rows, k, n, adapters, rank, kind="each"))
+
+
+@pytest.mark.parametrize("rows,pairs,rank", [(17001, False, 256), (17001, False, 250), (9001, True, 256), (9001, True, 250)])
+def test_low_rank_rows_in_several_passes(gpu, pkg, monkeypatch, rows, pairs, rank):
+    """Low-rank rows beyond 1 GiB. A tile of 128 rows has room for 128 entries of 128 x 256 columns, 8 MiB: 133 tiles are
+    128 and 5. One of 256 rows has room for 256 of 256 x 256, 32 MiB: 36 tiles are 32 and 4. (Rank 250 is stored as 256,
+    with up copied to rows of 256 in front of the first pass.)"""
+    if pairs:
+        monkeypatch.setenv("H3B_CTA_PAIRS_ALWAYS", "1")
+    case = Case(rows, 64, 64, 256, rank, kind="random")
+    got = case.run(gpu, pkg)
+    assert_within(got, *case.reference(), f"{rows} rows, rank {rank}")
+    assert np.array_equal(got, case.run(gpu, pkg))
