@@ -934,7 +934,10 @@ int ct_launch(h3_gpu *gpu, CrossArgs &args, const uint16_t *q, const uint16_t *k
         config.numAttrs = 1;
         cudaLaunchKernelEx(&config, h3b_cross_merge<D>, args);
     }
-    return h3b_launched(gpu, "cross_sdpa_bf16", H3B_SDPA);
+    /* the form of the call is part of its name in the op profile */
+    const char *name = GROUPS == 2 ? (pieces > 1 ? "cross_sdpa_bf16, two tiles, cut" : "cross_sdpa_bf16, two tiles")
+                                   : (pieces > 1 ? "cross_sdpa_bf16, one tile, cut" : "cross_sdpa_bf16, one tile");
+    return h3b_launched(gpu, name, H3B_SDPA);
 }
 
 bool cross_env_on(const char *name) {
@@ -1009,5 +1012,5 @@ extern "C" int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_
     const size_t smem = (size_t(head_dim) + kSimtThreads) * sizeof(float);
     h3b_cross_simt<<<dim3(query_rows, heads), kSimtThreads, smem, gpu->stream>>>(
         q, k, v, out, table, segment_count, query_rows, key_rows, heads, kv_heads, head_dim, scale);
-    return h3b_launched(gpu, "cross_sdpa_bf16", H3B_SDPA);
+    return h3b_launched(gpu, "cross_sdpa_bf16, any shape", H3B_SDPA);
 }
