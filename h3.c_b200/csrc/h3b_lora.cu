@@ -430,8 +430,8 @@ h3b_lora_down_few(const __grid_constant__ h3b_lora_task task) {
 
 /* The projection of few rows: D[weight row][x row] = W.x^T for 128 weight rows and the up to 128 rows of the call, the
  * weight streamed once through the M side of the instruction. K is split over the CTAs of a cluster so
- * that every SM pulls on the weight (42 weight tiles of n = 5,376 would leave 106 SMs idle); the last CTA
- * takes the entries' blocks too. Partial sums are joined through distributed shared memory in rank order.
+ * that every SM pulls on the weight (42 weight tiles of n = 5,376 would leave 106 SMs idle); the entries'
+ * blocks are dealt out over the CTAs of the cluster. Partial sums are joined through distributed shared memory in rank order.
  * Bound by the weight's bytes: one row, 7,168 -> 5,376, 77 MB in 16 us. */
 struct RowsArgs {
     h3b_lora_task task;
