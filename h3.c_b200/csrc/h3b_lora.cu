@@ -754,10 +754,13 @@ int lora_tensor_cores(h3_gpu *gpu, const h3b_lora_task &task, bool few, bool cap
         return h3b_fail(gpu, "linear_lora_bf16: cannot encode the tensor maps");
     /* By warps where that is the shorter way and there is no long weight stream to hide it behind (us, by warps / tensor
      * cores: 4 rows 1,024 -> 5,376 rank 16 8.6 / 11.7, 128 rows 15.1 / 17.5, rank 64 22.2 / 18.5; 2,048 -> 5,376 16
-     * rows 12.0 / 13.3; 2,688 -> 10,752 16 rows 18.9 / 17.0; 5,376 -> 5,376 64 rows 21.8 / 19.5), and for the smallest
-     * calls of all (1 row 5,376 -> 5,376 rank 16 16.0 / 16.8). */
+     * rows 12.0 / 13.3; 2,688 -> 10,752 16 rows 18.9 / 17.0; 5,376 -> 5,376 64 rows 21.8 / 19.5), and up to 8 CTAs (2
+     * stored sums each) beside any weight: more of them take SMs that the streaming kernel's clusters wait for. 1 row of
+     * rank 16 or 2 of rank 8, 8 CTAs: 5,376 -> 5,376 16.0 / 17.1, 7,168 -> 5,376 18.0 / 18.5, 14,336 -> 5,376 29.1 / 29.6,
+     * 5,376 -> 21,504 42.6 / 43.0, 2,688 -> 96,768 84.9 / 85.3; 1 row of rank 32 or 4 of rank 4, 16 CTAs: 24.5 / 17.5,
+     * 28.2 / 19.7, 46.1 / 29.5, 42.6 / 43.1, 84.8 / 85.4. */
     const uint64_t sums = uint64_t(task.rows) * task.rank;
-    if (few && (sums <= 16 || (sums <= 2048 && uint64_t(task.n) * task.k <= 12000000)))
+    if (few && (uint64_t(task.rows) * task.rank8 <= 16 || (sums <= 2048 && uint64_t(task.n) * task.k <= 12000000)))
         launch_cluster(gpu, h3b_lora_down_few, dim3(task.rows, task.rank8 / LF_SUMS), 32 * LF_WARPS, 1, 0, dependent, task);
     else
         launch_cluster(gpu, h3b_lora_down_tc, dim3(down_split, row_blocks, side), LR_THREADS, down_split, ring_smem(down.ring), dependent,
