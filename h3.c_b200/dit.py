@@ -268,6 +268,10 @@ class Dit:
         g, s, rows = self.gpu, self.s, self.active_rows
         if (adapters is not None or conditioning is not None) and self.exchange.world != 1:
             raise ValueError("adapters and conditioning are not combined with sequence parallelism")
+        if (adapters is not None or conditioning is not None) and rows != self.rows_local:
+            raise ValueError("adapters and conditioning are not combined with token reduction")
+        if conditioning is not None and (conditioning.rows != rows or not 0 <= block < len(conditioning.blocks)):
+            raise ValueError("conditioning must have these rows and keys and values for this block")
         if not adaln_ready:
             g.op("adaln_bf16", self.mod_attention, self.hidden, w.norm1, w.modulation, row_map,
                  rows, s.hidden, s.slots, 0, 1, s.eps)
