@@ -4,7 +4,11 @@
  * ascending; entry e has a block of tile_rows low-rank rows t (BF16, rank8 = rank rounded up to 8 columns,
  * zeros behind rank): scale[a] x.down[a]^T where the row's adapter is the entry's, zeros elsewhere. Then
  *   out tile = x.W^T + sum_e t_e . up[a_e]^T
- * is one accumulation on the tensor cores: the entries are more K blocks behind the projection's own. */
+ * is one accumulation on the tensor cores: the entries are more K blocks behind the projection's own.
+ *
+ * t is F32 until it is scaled and then rounded to BF16 once, since both operands of an instruction have one type
+ * and up is BF16: 2^-8 of |t| . |up| at most, of a term that is small beside x.W^T. A second block of what the
+ * rounding left would take that to 2^-16 for twice the entries' K blocks; the result's own rounding is 2^-8 of all of it. */
 #pragma once
 
 #include "h3b_common.cuh"

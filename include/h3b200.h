@@ -472,7 +472,10 @@ int h3x_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor
  * must be 0). Segments may share key rows and may leave gaps anywhere (states padded to one length);
  * their query rows must not overlap. Query rows in no segment are left as they were; rows of a
  * segment past query_rows or key_rows are ignored; what padding rows hold (infinities and NaN
- * included) never reaches an output. heads must divide by kv_heads; head_dim up to 512 (64 and 128 with
+ * included) never reaches an output. A key whose score is -inf has the probability 0 (which times a value
+ * that is not finite is NaN), and a row without any other key is zero. On the tensor cores scores
+ * (query . key * scale) have to stay below 2^29 in magnitude: from there the step of F32 next to them no
+ * longer fits the exponent of a probability. heads must divide by kv_heads; head_dim up to 512 (64 and 128 with
  * 16-byte aligned tensors and scale > 0 run on the tensor cores). output may be the query tensor
  * itself; it must not overlap key or value. */
 int h3x_cross_sdpa_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,

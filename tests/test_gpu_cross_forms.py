@@ -313,3 +313,27 @@ def test_hopeless_keys_in_every_form(profiled, form, dim, lengths, heads, want_f
     assert np.isnan(wide(got[:rows, :, ::2])).all()
     assert_within(got[sample][:, :, 1::2], want[:, :, 1::2], tol[:, :, 1::2], want_form)
     assert np.isfinite(wide(got[rows:])).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lengths,heads,want_form", [
+    ([(1, 4096)], 4, "one tile, cut"), ([(300, 500)], 4, "one tile"), ([(1000, 500)], 112, "two tiles")])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_two_to_the_28(profiled, form, dim, lengths, heads, want_form, sign):
+    """Queries and keys whose scores are exact in F32, up to 2^28 in magnitude with steps of 2^21: the largest takes all.
+    The kernel's reference is off from it by up to half a step of 2^29 (2^-24 of it: 32), which has to cancel."""
+    (rows, keys), = lengths
+    case = Case([[0, rows, 0, keys]], heads, heads, dim)
+    exact = lambda values: (values.astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
+    case.q = exact(np.full(case.q.size, sign * 4096.0))
+    rng = np.random.default_rng(keys)
+    c = np.r_[np.arange(keys - 1) % 127 + 1, 128] * (2.0 ** 16 / dim / 128)      # dot: 4096 * dim * c = 2^21 * (1 .. 128)
+    if sign < 0:                                                               # the largest score is the smallest in magnitude
+        c = np.where(np.arange(keys) == keys - 1, 64.0, 64 + np.arange(keys) % 64 + 1) * (2.0 ** 16 / dim / 128)
+    order = rng.permutation(keys)
+    case.k = exact(np.repeat(c[order], heads * dim))
+    got = wide(case.run(profiled, 1.0)).reshape(rows, heads, dim)
+    assert form() == want_form
+    want = wide(case.v).reshape(keys, heads, dim)[np.argmax(order)]
+    # the probability is rounded to BF16, its sum is not; the result is rounded to BF16
+    assert (np.abs(got - want) <= (2.0 ** -8 + 2.0 ** -8 + 2.0 ** -16 + 2.0 ** -20) * np.abs(want)).all()
