@@ -447,7 +447,8 @@ int h3x_linear_swiglu_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tens
  * the tensor cores. BF16: input [rows][input_dim], weight [output_dim][input_dim], bias [output_dim] or
  * NULL, down [adapters][rank][input_dim], up [adapters][output_dim][rank], output [rows][output_dim].
  * scale is F32 [adapters] or NULL (all 1); row_adapter is U32 [rows] or NULL (every row has adapter 0).
- * Adapters of a smaller rank are padded with zeros to `rank`. Rows of one request need not be
+ * Adapters of a smaller rank are padded with zeros to `rank`; a rank that is not a multiple of 8 has up of
+ * all adapters copied to padded rows in every call. Rows of one request need not be
  * contiguous; a row never depends on another row's adapter, whatever that adapter's weights hold: where
  * rows of several adapters share a tile and something in it is not finite, that is computed again at the
  * end of the kernel, which takes its time (one of 16 adapters all infinities, 1,003 rows 5,120 -> 5,376:
